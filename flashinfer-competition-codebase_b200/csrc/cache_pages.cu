@@ -1,0 +1,574 @@
+// cache_pages.cu — the pages of a cache: slots of a pooled recurrent state, pages of a
+// paged key-value cache.  A pool is [num_pages, page bytes] with any pitch between pages;
+// several pools (layers, keys and values) that share one page numbering go through one call.
+//
+//   copy      pools[dst[i]] = pools[src[i]] for all i at once: every source is read as it
+//             was before the call, of equal dst the last pair wins
+//   fork      rows of a block table become children of rows, with reference counts; a
+//             partly filled last page is copied for every child but the first
+//   compact   live pages behind the first num_live move into the holes before it
+//   alloc     the lowest free pages; free: one reference less per listed page
+//
+// A page is free when its reference count is <= 0.  All results are defined by order of
+// index (lowest page first, lowest row first), so they do not depend on scheduling.
+
+#include <string.h>
+
+#include "serving_common.cuh"
+
+namespace {
+
+using namespace gdn_serving;
+
+constexpr int kMaxPools = 32;
+constexpr int kMaxPairs = 4096;
+constexpr int kThreads = 256;
+constexpr int kVecs = 16;          // 16-byte vectors a thread holds: 64 KB per CTA
+
+struct Pools {
+  char* base[kMaxPools];
+  long long bytes[kMaxPools];      // of one page
+  long long pitch[kMaxPools];      // from page to page
+  int count;
+  int num_pages;
+};
+
+// ------------------------------------------------------------------ simultaneous copy
+//
+// A CTA takes one column (the same bytes of every page), reads it from all sources into
+// registers, waits for all its threads, and writes it to all destinations.  No other CTA
+// touches that column, so sources that are destinations too (a permutation of beams, a
+// cycle) are read before they are overwritten, without a second buffer: 2 x bytes moved.
+
+struct CopyArgs {
+  Pools pools;
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t* bad;
+  int n;
+  int hash;                        // entries of the hash table, a power of two >= 2 n
+};
+
+template <typename U>
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyArgs p) {
+  extern __shared__ int32_t smem[];
+  int32_t* key = smem;                    // [hash] dst of an entry
+  int32_t* last = smem + p.hash;          // [hash] its last pair
+  int32_t* list = smem + 2 * p.hash;      // [2 n] active pairs: src, dst
+  __shared__ int active, bad;
+  const int tid = threadIdx.x, P = p.pools.num_pages;
+  for (int i = tid; i < p.hash; i += kThreads) {
+    key[i] = -1;
+    last[i] = -1;
+  }
+  if (tid == 0) active = bad = 0;
+  __syncthreads();
+  auto slot_of = [&](int d) {
+    uint32_t at = static_cast<uint32_t>(d) * 2654435761u & (p.hash - 1);
+    while (true) {                        // at most n of >= 2 n entries are taken
+      const int k = atomicCAS(&key[at], -1, d);
+      if (k == -1 || k == d) return at;
+      at = (at + 1) & (p.hash - 1);
+    }
+  };
+  for (int i = tid; i < p.n; i += kThreads) {
+    const int s = p.src[i], d = p.dst[i];
+    if (s < 0 || d < 0) continue;
+    if (s >= P || d >= P) {
+      atomicAdd(&bad, 1);
+      continue;
+    }
+    atomicMax(&last[slot_of(d)], i);
+  }
+  __syncthreads();
+  for (int i = tid; i < p.n; i += kThreads) {
+    const int s = p.src[i], d = p.dst[i];
+    if (s < 0 || d < 0 || s >= P || d >= P || s == d) continue;
+    if (last[slot_of(d)] != i) continue;
+    const int at = atomicAdd(&active, 1);
+    list[2 * at] = s;
+    list[2 * at + 1] = d;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0 && p.bad && bad) atomicAdd(p.bad, bad);
+  const int n = active;
+  if (n == 0) return;
+  // vectors of one page per column: as many as the registers hold, fewer when that would
+  // leave CTAs without a column
+  int shift = 0;
+  while ((2 << shift) * n <= kThreads * kVecs) ++shift;
+  long long total = 0;
+  for (int i = 0; i < p.pools.count; ++i) total += p.pools.bytes[i] / static_cast<int>(sizeof(U));
+  while (shift > 5 && (total >> shift) < gridDim.x) --shift;
+  long long item = blockIdx.x;
+  for (int pool = 0; pool < p.pools.count; ++pool) {
+    const long long vecs = p.pools.bytes[pool] / static_cast<int>(sizeof(U));
+    const long long cols = (vecs + (1ll << shift) - 1) >> shift;
+    for (; item < cols; item += gridDim.x) {
+      U v[kVecs];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int f = tid + k * kThreads, i = f >> shift;
+        const long long at = (item << shift) + (f & ((1 << shift) - 1));
+        if (i < n && at < vecs)
+          v[k] = reinterpret_cast<const U*>(p.pools.base[pool] + list[2 * i] * p.pools.pitch[pool])[at];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int f = tid + k * kThreads, i = f >> shift;
+        const long long at = (item << shift) + (f & ((1 << shift) - 1));
+        if (i < n && at < vecs)
+          reinterpret_cast<U*>(p.pools.base[pool] + list[2 * i + 1] * p.pools.pitch[pool])[at] = v[k];
+      }
+    }
+    item -= cols;
+  }
+}
+
+// ------------------------------------------------------------------ disjoint moves
+//
+// Pairs whose destinations are no other pair's source (fork, compact): a work item is a
+// segment of one pair's page, and any CTA may take it at any time.
+
+struct MoveArgs {
+  Pools pools;
+  const int32_t* src;              // < 0: no pair
+  const int32_t* dst;
+  const int32_t* count;            // device count of pairs, or null: n
+  int n;
+};
+
+template <typename U>
+__global__ void __launch_bounds__(kThreads) move_pages_kernel(const __grid_constant__ MoveArgs p) {
+  const long long n = p.count ? *p.count : p.n;
+  long long item = blockIdx.x;
+  for (int pool = 0; pool < p.pools.count; ++pool) {
+    const long long vecs = p.pools.bytes[pool] / static_cast<int>(sizeof(U));
+    const long long segs = (vecs + kThreads * kVecs - 1) / (kThreads * kVecs);
+    for (; item < n * segs; item += gridDim.x) {
+      const long long pair = item / segs, seg = item % segs;
+      const int s = p.src[pair], d = p.dst[pair];
+      if (s < 0 || d < 0) continue;
+      const U* from = reinterpret_cast<const U*>(p.pools.base[pool] + s * p.pools.pitch[pool]);
+      U* to = reinterpret_cast<U*>(p.pools.base[pool] + d * p.pools.pitch[pool]);
+      U v[kVecs];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const long long at = (seg * kVecs + k) * kThreads + threadIdx.x;
+        if (at < vecs) v[k] = from[at];
+      }
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const long long at = (seg * kVecs + k) * kThreads + threadIdx.x;
+        if (at < vecs) to[at] = v[k];
+      }
+    }
+    item -= n * segs;
+  }
+}
+
+// ------------------------------------------------------------------ plans (one CTA)
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive prefix sum over the CTA; `total` gets the sum.  Every thread calls it.
+__device__ int block_scan(int x, int& total) {
+  __shared__ int part[32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int y = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
+  }
+  __syncthreads();                 // the last call's readers of part are done
+  if (lane == 31) part[warp] = y;
+  __syncthreads();
+  if (warp == 0) {
+    int w = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += z;
+    }
+    part[lane] = w;
+  }
+  __syncthreads();
+  total = part[31];
+  return y - x + (warp ? part[warp - 1] : 0);
+}
+
+// Gives the k-th wanting row (ascending) the k-th free page (ascending), with reference
+// count 1; calls give(row, page) for each wanting row, page -1 when there are too few.
+template <typename Wants, typename Give>
+__device__ void assign_free(int32_t* refcounts, int P, int n, int32_t* row_of, Wants wants, Give give) {
+  int needed = 0, total;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    const int w = i < n && wants(i);
+    const int at = needed + block_scan(w, total);
+    if (w) row_of[at] = i;
+    needed += total;
+  }
+  __syncthreads();
+  int found = 0;
+  for (int p0 = 0; p0 < P && found < needed; p0 += kPlanThreads) {
+    const int page = p0 + threadIdx.x;
+    const int f = page < P && refcounts[page] <= 0;
+    const int at = found + block_scan(f, total);
+    if (f && at < needed) {
+      refcounts[page] = 1;
+      give(row_of[at], page);
+    }
+    found += total;
+  }
+  for (int k = found + threadIdx.x; k < needed; k += kPlanThreads) give(row_of[k], -1);
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+alloc_pages_kernel(int32_t* refcounts, int P, const uint8_t* need, int n, int32_t* pages,
+                   int32_t* row_of) {
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) pages[i] = -1;
+  __syncthreads();
+  assign_free(refcounts, P, n, row_of, [&](int i) { return need[i] != 0; },
+              [&](int i, int page) { pages[i] = page; });
+}
+
+__global__ void free_pages_kernel(int32_t* refcounts, int P, const int32_t* pages, long long n,
+                                  int32_t* bad) {
+  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n; i += step) {
+    const int page = pages[i];
+    if (page < 0) continue;
+    // one reference less; a page that has none keeps its count (the sum of the decrements
+    // and of the ones taken back is the same in every order)
+    if (page >= P || atomicSub(&refcounts[page], 1) <= 0) {
+      if (page < P) atomicAdd(&refcounts[page], 1);
+      if (bad) atomicAdd(bad, 1);
+    }
+  }
+}
+
+struct ForkArgs {
+  const int32_t* tables;           // [rows_in, width], row stride
+  const int32_t* lens;             // [rows_in]
+  const int32_t* parents;          // [rows_out]
+  int32_t* refcounts;              // [P]
+  int32_t* new_tables;             // [rows_out, width]
+  int32_t* new_lens;               // [rows_out]
+  int32_t* src;                    // workspace [rows_out]: page to copy, or -1
+  int32_t* dst;                    // workspace [rows_out]: its copy
+  int32_t* row_of;                 // workspace [rows_out]
+  int32_t* bad;
+  long long stride;
+  int rows_in, rows_out, width, P, page_size;
+};
+
+// CTA r: the references of input row r, and output row r.
+__global__ void __launch_bounds__(kThreads) fork_rows_kernel(ForkArgs p) {
+  const int r = blockIdx.x, tid = threadIdx.x;
+  __shared__ int count, earlier;
+  if (tid == 0) count = earlier = 0;
+  __syncthreads();
+  const int parent = r < p.rows_out ? p.parents[r] : -1;
+  const bool child = parent >= 0 && parent < p.rows_in;
+  int c = 0, e = 0;
+  for (int i = tid; i < p.rows_out; i += kThreads) {
+    const int q = p.parents[i];
+    c += q == r;
+    e |= i < r && q == parent;
+  }
+  if (c) atomicAdd(&count, c);
+  if (e) earlier = 1;
+  __syncthreads();
+  auto tokens = [&](int row) {
+    const int n = p.lens[row], cap = p.width * p.page_size;
+    return n < 0 ? 0 : n > cap ? cap : n;
+  };
+  if (r < p.rows_in && count != 1) {
+    const int n = tokens(r), full = n / p.page_size, part = n % p.page_size != 0;
+    const int32_t* row = p.tables + r * p.stride;
+    for (int j = tid; j < full + part; j += kThreads) {
+      const int page = row[j], delta = j < full ? count - 1 : (count ? 0 : -1);
+      if (page >= 0 && page < p.P && delta) atomicAdd(&p.refcounts[page], delta);
+    }
+  }
+  if (r < p.rows_out) {
+    const int n = child ? tokens(parent) : 0, full = n / p.page_size, part = n % p.page_size != 0;
+    const int32_t* row = p.tables + (child ? parent : 0) * p.stride;
+    int32_t* out = p.new_tables + static_cast<long long>(r) * p.width;
+    for (int j = tid; j < p.width; j += kThreads) out[j] = j < full + part ? row[j] : -1;
+    if (tid == 0) {
+      p.new_lens[r] = n;
+      const int page = part ? row[full] : -1;
+      p.src[r] = (earlier && page >= 0 && page < p.P) ? page : -1;
+      p.dst[r] = -1;
+      if (parent >= p.rows_in && p.bad) atomicAdd(p.bad, 1);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs p) {
+  assign_free(p.refcounts, p.P, p.rows_out, p.row_of, [&](int i) { return p.src[i] >= 0; },
+              [&](int i, int page) {
+                p.dst[i] = page;
+                p.new_tables[static_cast<long long>(i) * p.width + p.new_lens[i] / p.page_size] = page;
+                if (page < 0 && p.bad) atomicAdd(p.bad, 1);
+              });
+}
+
+struct CompactArgs {
+  int32_t* refcounts;              // [P]
+  int32_t* remap;                  // [P]
+  int32_t* live;                   // [1]
+  int32_t* src;                    // workspace [P / 2 + 1]
+  int32_t* dst;
+  int32_t* count;                  // workspace [1]
+  int P;
+};
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs p) {
+  int c = 0, live;
+  for (int i = threadIdx.x; i < p.P; i += kPlanThreads) c += p.refcounts[i] > 0;
+  block_scan(c, live);
+  int movers = 0, holes = 0, total;
+  for (int i0 = 0; i0 < p.P; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    const bool in = i < p.P, on = in && p.refcounts[i] > 0;
+    const int mv = on && i >= live, ho = in && !on && i < live;
+    const int am = movers + block_scan(mv, total);
+    movers += total;
+    const int ah = holes + block_scan(ho, total);
+    holes += total;
+    if (mv) p.src[am] = i;
+    if (ho) p.dst[ah] = i;
+    if (in) p.remap[i] = on ? i : -1;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < movers; k += kPlanThreads) {
+    const int s = p.src[k], d = p.dst[k];
+    p.remap[s] = d;
+    p.refcounts[d] = p.refcounts[s];
+    p.refcounts[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *p.live = live;
+    *p.count = movers;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+remap_tables_kernel(int32_t* tables, long long n, const int32_t* remap, int P) {
+  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n; i += step) {
+    const int page = tables[i];
+    if (page >= 0 && page < P) tables[i] = remap[page];
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+int check_pools(void* const* pools, const int64_t* bytes, const int64_t* pitch, int num_pools,
+                int num_pages, Pools& out, int& unit) {
+  if (num_pools < 0 || num_pages < 1) return GDN_ERR_SHAPE;
+  if (num_pools > kMaxPools) return GDN_ERR_LIMIT;
+  if (num_pools > 0 && (!pools || !bytes || !pitch)) return GDN_ERR_NULL;
+  memset(&out, 0, sizeof(out));
+  out.count = num_pools;
+  out.num_pages = num_pages;
+  unit = 16;
+  for (int i = 0; i < num_pools; ++i) {
+    if (!pools[i]) return GDN_ERR_NULL;
+    if (bytes[i] < 1) return GDN_ERR_SHAPE;
+    if (pitch[i] < bytes[i]) return GDN_ERR_ALIAS;     // pages of one pool overlap
+    out.base[i] = static_cast<char*>(pools[i]);
+    out.bytes[i] = bytes[i];
+    out.pitch[i] = pitch[i];
+    const uintptr_t all = reinterpret_cast<uintptr_t>(pools[i]) | static_cast<uintptr_t>(bytes[i]) |
+                          static_cast<uintptr_t>(pitch[i]);
+    while (all % unit) unit /= 4;
+    // two pools may interleave (key and value halves of one buffer) but not share a byte
+    for (int j = 0; j < i; ++j) {
+      if (!overlaps(out.base[i], (num_pages - 1) * pitch[i] + bytes[i], out.base[j],
+                    (num_pages - 1) * pitch[j] + bytes[j]))
+        continue;
+      if (pitch[i] != pitch[j]) return GDN_ERR_ALIAS;
+      int64_t off = (out.base[i] - out.base[j]) % pitch[i];
+      if (off < 0) off += pitch[i];
+      if (off < bytes[j] || off + bytes[i] > pitch[i]) return GDN_ERR_ALIAS;
+    }
+  }
+  return GDN_OK;
+}
+
+// enough CTAs for the vectors to move, at most two per SM
+unsigned grid_for(const Pools& pools, int unit, long long pairs) {
+  long long vecs = 0;
+  for (int i = 0; i < pools.count; ++i) vecs += pools.bytes[i] / unit;
+  long long ctas = (vecs * pairs + kThreads - 1) / kThreads;
+  return static_cast<unsigned>(ctas < 1 ? 1 : ctas > 2 * 148 ? 2 * 148 : ctas);
+}
+
+cudaError_t launch_moves(const MoveArgs& a, int unit, unsigned grid, cudaStream_t st) {
+  if (unit == 16) move_pages_kernel<uint4><<<grid, kThreads, 0, st>>>(a);
+  else if (unit == 4) move_pages_kernel<uint32_t><<<grid, kThreads, 0, st>>>(a);
+  else move_pages_kernel<uint8_t><<<grid, kThreads, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int gdn_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t* page_pitch,
+                   int num_pools, int num_pages, const int32_t* src, const int32_t* dst, int n,
+                   int32_t* bad_index_count, void* stream) {
+  CopyArgs a{};
+  int unit = 16;
+  const int rc = check_pools(pools, page_bytes, page_pitch, num_pools, num_pages, a.pools, unit);
+  if (rc != GDN_OK) return rc;
+  if (n < 0) return GDN_ERR_SHAPE;
+  if (n > kMaxPairs) return GDN_ERR_LIMIT;
+  if (n == 0 || num_pools == 0) return GDN_OK;
+  if (!src || !dst) return GDN_ERR_NULL;
+  if (!aligned(src, 4) || !aligned(dst, 4) || !aligned(bad_index_count, 4)) return GDN_ERR_ALIGN;
+  a.src = src;
+  a.dst = dst;
+  a.bad = bad_index_count;
+  a.n = n;
+  a.hash = 64;
+  while (a.hash < 2 * n) a.hash *= 2;
+  const size_t smem = (2 * static_cast<size_t>(a.hash) + 2 * static_cast<size_t>(n)) * 4;
+  const unsigned grid = grid_for(a.pools, unit, n);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) {
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+      return GDN_ERR_LAUNCH;
+    kernel<<<grid, kThreads, smem, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+  };
+  return unit == 16 ? go(copy_pages_kernel<uint4>)
+                    : unit == 4 ? go(copy_pages_kernel<uint32_t>) : go(copy_pages_kernel<uint8_t>);
+}
+
+int gdn_alloc_pages(int32_t* refcounts, int num_pages, const uint8_t* need, int n, int32_t* pages,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (num_pages < 1 || n < 0) return GDN_ERR_SHAPE;
+  if (n == 0) return GDN_OK;
+  if (!refcounts || !need || !pages || !workspace) return GDN_ERR_NULL;
+  if (!aligned(refcounts, 4) || !aligned(pages, 4) || !aligned(workspace, 4)) return GDN_ERR_ALIGN;
+  if (workspace_bytes < static_cast<size_t>(n) * 4) return GDN_ERR_SHAPE;
+  alloc_pages_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      refcounts, num_pages, need, n, pages, static_cast<int32_t*>(workspace));
+  return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+}
+
+int gdn_free_pages(int32_t* refcounts, int num_pages, const int32_t* pages, int64_t n,
+                   int32_t* bad_index_count, void* stream) {
+  if (num_pages < 1 || n < 0) return GDN_ERR_SHAPE;
+  if (n == 0) return GDN_OK;
+  if (!refcounts || !pages) return GDN_ERR_NULL;
+  if (!aligned(refcounts, 4) || !aligned(pages, 4) || !aligned(bad_index_count, 4))
+    return GDN_ERR_ALIGN;
+  const int64_t ctas = (n + kThreads - 1) / kThreads;
+  free_pages_kernel<<<static_cast<unsigned>(ctas > 148 * 8 ? 148 * 8 : ctas), kThreads, 0,
+                      static_cast<cudaStream_t>(stream)>>>(refcounts, num_pages, pages, n,
+                                                           bad_index_count);
+  return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+}
+
+int gdn_fork_pages(const int32_t* block_tables, int64_t table_stride, const int32_t* seq_lens,
+                   const int32_t* parents, int32_t* refcounts, int32_t* new_tables,
+                   int32_t* new_lens, int rows_in, int rows_out, int table_width, int num_pages,
+                   int page_size, void* const* pools, const int64_t* page_bytes,
+                   const int64_t* page_pitch, int num_pools, void* workspace,
+                   size_t workspace_bytes, int32_t* bad_index_count, void* stream) {
+  MoveArgs m{};
+  int unit = 16;
+  const int rc = check_pools(pools, page_bytes, page_pitch, num_pools, num_pages, m.pools, unit);
+  if (rc != GDN_OK) return rc;
+  if (rows_in < 0 || rows_out < 0 || table_width < 0 || page_size < 1) return GDN_ERR_SHAPE;
+  if (static_cast<long long>(table_width) * page_size > 0x7fffffffLL || table_stride < 0)
+    return GDN_ERR_SHAPE;
+  if (rows_in == 0 && rows_out == 0) return GDN_OK;
+  if (!refcounts || (rows_in > 0 && !seq_lens) || (rows_out > 0 && (!parents || !new_lens || !workspace)))
+    return GDN_ERR_NULL;
+  if (table_width > 0 && ((rows_in > 0 && !block_tables) || (rows_out > 0 && !new_tables)))
+    return GDN_ERR_NULL;
+  if (!aligned(block_tables, 4) || !aligned(seq_lens, 4) || !aligned(parents, 4) ||
+      !aligned(refcounts, 4) || !aligned(new_tables, 4) || !aligned(new_lens, 4) ||
+      !aligned(workspace, 4) || !aligned(bad_index_count, 4))
+    return GDN_ERR_ALIGN;
+  if (workspace_bytes < 12 * static_cast<size_t>(rows_out)) return GDN_ERR_SHAPE;
+  if (table_width > 0 && rows_in > 0 && rows_out > 0 &&
+      overlaps(block_tables, ((rows_in - 1) * table_stride + table_width) * 4, new_tables,
+               static_cast<size_t>(rows_out) * table_width * 4))
+    return GDN_ERR_ALIAS;
+  if (rows_in > 0 && rows_out > 0 &&
+      overlaps(seq_lens, static_cast<size_t>(rows_in) * 4, new_lens, static_cast<size_t>(rows_out) * 4))
+    return GDN_ERR_ALIAS;
+  ForkArgs p{};
+  p.tables = block_tables; p.lens = seq_lens; p.parents = parents; p.refcounts = refcounts;
+  p.new_tables = new_tables; p.new_lens = new_lens;
+  p.src = static_cast<int32_t*>(workspace);
+  p.dst = p.src + rows_out;
+  p.row_of = p.dst + rows_out;
+  p.bad = bad_index_count; p.stride = table_stride;
+  p.rows_in = rows_in; p.rows_out = rows_out; p.width = table_width; p.P = num_pages;
+  p.page_size = page_size;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  fork_rows_kernel<<<rows_in > rows_out ? rows_in : rows_out, kThreads, 0, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
+  if (rows_out == 0) return GDN_OK;
+  fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
+  if (num_pools == 0) return GDN_OK;
+  m.src = p.src;
+  m.dst = p.dst;
+  m.n = rows_out;
+  return launch_moves(m, unit, grid_for(m.pools, unit, rows_out), st) == cudaSuccess ? GDN_OK
+                                                                                     : GDN_ERR_LAUNCH;
+}
+
+int gdn_compact_pages(int32_t* refcounts, int num_pages, int32_t* block_tables,
+                      int64_t table_entries, int32_t* remap, int32_t* num_live,
+                      void* const* pools, const int64_t* page_bytes, const int64_t* page_pitch,
+                      int num_pools, void* workspace, size_t workspace_bytes, void* stream) {
+  MoveArgs m{};
+  int unit = 16;
+  const int rc = check_pools(pools, page_bytes, page_pitch, num_pools, num_pages, m.pools, unit);
+  if (rc != GDN_OK) return rc;
+  if (table_entries < 0) return GDN_ERR_SHAPE;
+  if (!refcounts || !remap || !num_live || !workspace || (table_entries > 0 && !block_tables))
+    return GDN_ERR_NULL;
+  if (!aligned(refcounts, 4) || !aligned(block_tables, 4) || !aligned(remap, 4) ||
+      !aligned(num_live, 4) || !aligned(workspace, 4))
+    return GDN_ERR_ALIGN;
+  const size_t half = static_cast<size_t>(num_pages) / 2 + 1;
+  if (workspace_bytes < (2 * half + 1) * 4) return GDN_ERR_SHAPE;
+  CompactArgs p{};
+  p.refcounts = refcounts; p.remap = remap; p.live = num_live; p.P = num_pages;
+  p.src = static_cast<int32_t*>(workspace);
+  p.dst = p.src + half;
+  p.count = p.dst + half;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
+  if (table_entries > 0) {
+    const int64_t ctas = (table_entries + kThreads - 1) / kThreads;
+    remap_tables_kernel<<<static_cast<unsigned>(ctas > 148 * 8 ? 148 * 8 : ctas), kThreads, 0, st>>>(
+        block_tables, table_entries, remap, num_pages);
+    if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
+  }
+  if (num_pools == 0) return GDN_OK;
+  m.src = p.src;
+  m.dst = p.dst;
+  m.count = p.count;
+  return launch_moves(m, unit, grid_for(m.pools, unit, static_cast<long long>(half)), st) == cudaSuccess
+             ? GDN_OK : GDN_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -23,6 +23,15 @@ from .ops import (  # noqa: F401
     kernel_cuda_b200,
     load_algo_functions,
 )
+from .serving import (  # noqa: F401
+    alloc_pages,
+    beam_select,
+    compact_pages,
+    copy_pages,
+    fork_pages,
+    free_pages,
+    paged_attention_decode,
+)
 
 __all__ = [
     "GdnError",
@@ -43,4 +52,11 @@ __all__ = [
     "ALGO_ENTRY_POINTS",
     "ALGO_NO_DPS",
     "load_algo_functions",
+    "paged_attention_decode",
+    "beam_select",
+    "copy_pages",
+    "fork_pages",
+    "compact_pages",
+    "alloc_pages",
+    "free_pages",
 ]

@@ -18,6 +18,7 @@ _I = ctypes.c_int
 _D = ctypes.c_double
 _U = ctypes.c_uint32
 _Z = ctypes.c_size_t
+_L = ctypes.c_int64
 
 # Every function declared in include/gdn_b200.h with its ctypes signature.
 SIGNATURES = {
@@ -87,9 +88,32 @@ SIGNATURES = {
          _I, _I, _I, _P],
     ),
     "gdn_interleave_heads": (_I, [_P, _P, _I, _I, _I, _I, _P]),
+    "gdn_paged_attention_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "gdn_paged_attention_decode": (
+        _I,
+        [_P, _P, _P, _P, _P, _P, _P, _D, _I, _I, _P, _P, _P, _Z, _I, _I, _I, _I, _I, _I, _I, _I,
+         _L, _P, _P, _P, _P],
+    ),
+    "gdn_beam_select_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "gdn_beam_select": (
+        _I,
+        [_P, _I, _L, _L, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P],
+    ),
+    "gdn_copy_pages": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _P, _P]),
+    "gdn_alloc_pages": (_I, [_P, _I, _P, _I, _P, _P, _Z, _P]),
+    "gdn_free_pages": (_I, [_P, _I, _P, _L, _P, _P]),
+    "gdn_fork_pages": (
+        _I,
+        [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _P, _Z, _P, _P],
+    ),
+    "gdn_compact_pages": (_I, [_P, _I, _P, _L, _P, _P, _P, _P, _P, _I, _P, _Z, _P]),
 }
 
 ABI_VERSION = 1
+
+DTYPE_BF16 = 0
+DTYPE_FP16 = 1
+DTYPE_FP32 = 2
 
 GDN_OK = 0
 GDN_ERR_NULL = -1

@@ -22,7 +22,8 @@ INCLUDE_DIR = os.path.join(os.path.dirname(os.path.dirname(PKG_DIR)), "include")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libgdn_b200.so")
 
-SOURCES = ["gdn_decode.cu", "gdn_prefill_chunked.cu", "gdn_prefill_wy.cu"]
+SOURCES = ["gdn_decode.cu", "gdn_prefill_chunked.cu", "gdn_prefill_wy.cu",
+           "paged_attention.cu", "beam_select.cu", "cache_pages.cu"]
 TVM_LIB_PATH = os.path.join(LIB_DIR, "libgdn_b200_tvm.so")
 # measurement-only kernels of the benchmark (the state round-trip floor), kept out of
 # the decode library
@@ -35,6 +36,7 @@ NVCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-Xptxas", "-v",
+    "--threads", "0",
     "-shared",
     "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden",
@@ -55,6 +57,7 @@ def _sources():
 
 def _deps():
     return _sources() + [os.path.join(SRC_DIR, "tc_common.cuh"),
+                         os.path.join(SRC_DIR, "serving_common.cuh"),
                          os.path.join(INCLUDE_DIR, "gdn_b200.h"), os.path.abspath(__file__)]
 
 

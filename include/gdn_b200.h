@@ -5,8 +5,9 @@
  * the fused T=1 decode step, the pooled-state (continuous batching) step,
  * the multi-token (speculative verify) step, the bf16-state variant, the
  * tensor-parallel step that stores its outputs into every rank's buffer
- * over NVLink, and the head interleave used after an NCCL all-gather.  No
- * function here allocates memory: the caller owns every buffer.  No
+ * over NVLink, the head interleave used after an NCCL all-gather, and the
+ * serving operators around the step (paged decode attention, beam selection,
+ * cache pages; their section gives their layouts).  No function here allocates memory: the caller owns every buffer.  No
  * function synchronises the host: work is enqueued on the given stream
  * (NULL = the legacy default stream).
  *
@@ -35,6 +36,7 @@
 #ifndef GDN_B200_H
 #define GDN_B200_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -457,6 +459,143 @@ GDN_API int gdn_decode_tp_static(const gdn_bf16* q, const gdn_bf16* k, const gdn
  */
 GDN_API int gdn_interleave_heads(const gdn_bf16* gathered, gdn_bf16* output,
                          int world, int rows, int HVl, int V, void* stream);
+
+/*
+ * Serving operators around the decode step.  No counterpart in the reference, which
+ * decodes GDN layers only; they are what a server of a stack with GDN layers runs beside
+ * gdn_decode_pooled: its attention layers' decode step, beam search, and the upkeep of
+ * the caches.
+ *
+ * Element types of their tensors:
+ */
+#define GDN_DTYPE_BF16 0
+#define GDN_DTYPE_FP16 1
+#define GDN_DTYPE_FP32 2
+
+/*
+ * Softmax attention of one new token per sequence over a paged key-value cache.
+ *
+ *   q, output      [B, 1, HQ, D]   bf16 or fp16 (`dtype`), D in {64, 128, 256}
+ *   k_cache, v_cache  pages of page_size tokens; k_strides / v_strides = element strides
+ *                  of (page, token, head), each a multiple of 8; D is contiguous.  So
+ *                  [pages, tokens, HKV, D], [pages, HKV, tokens, D] and views of an
+ *                  interleaved buffer all fit.
+ *   block_tables   [B, table_width] int32, row stride table_stride: entry t / page_size is
+ *                  the page of token t
+ *   seq_lens       [B] int32: tokens of the sequence, the new one included
+ *   k_new, v_new   [B, 1, HKV, D] or both NULL: the new token's rows.  They are attended to
+ *                  as token seq_lens[b]-1 and stored into its place in the cache.
+ *   lse            [B, HQ] fp32 or NULL: ln(sum exp(scale * q.k))
+ * Query head h reads key-value head h / (HQ / HKV).  scale == 0 selects 1/sqrt(D).
+ * window > 0 limits the visible tokens to the first num_sinks and the last `window`.
+ *  - seq_lens[b] <= 0 (a padding row): output 0, lse -inf, nothing stored.
+ *  - A table entry < 0 hides its tokens; one >= num_pages does too and is counted once per
+ *    sequence in *bad_index_count (int32, may be NULL).  The new token is seen even so, but
+ *    not stored.  A row that sees nothing gets output 0, lse -inf.
+ *  - seq_lens[b] > table_width * page_size is counted, cut to that, and the new token is
+ *    neither seen nor stored.
+ * What a cache holds behind a sequence's last token is not read into the result (NaNs
+ * there are harmless).  The page of the last token must belong to this sequence alone;
+ * all other pages may be shared.  `workspace`: gdn_paged_attention_workspace_bytes bytes,
+ * 16-byte aligned, contents ignored and overwritten.  output may not overlap q or the caches.
+ */
+GDN_API size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D,
+                                                   int max_tokens);
+GDN_API int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
+                                       const int32_t* block_tables, const int32_t* seq_lens,
+                                       const void* k_new, const void* v_new, double scale,
+                                       int window, int num_sinks, void* output, float* lse,
+                                       void* workspace, size_t workspace_bytes, int dtype,
+                                       int B, int HQ, int HKV, int D, int num_pages,
+                                       int page_size, int table_width, int64_t table_stride,
+                                       const int64_t* k_strides, const int64_t* v_strides,
+                                       int32_t* bad_index_count, void* stream);
+
+/*
+ * Beam search's selection over beams and vocabulary.
+ *
+ *   logits [B, K, V] bf16, fp16 or fp32, element strides (stride_batch, stride_beam, 1)
+ *   scores [B, K] fp32 cumulative log-probabilities; finished [B, K] bytes or NULL
+ * Candidate (i, t) has score scores[i] + logits[i, t] - ln(sum_t exp(logits[i, t])); a
+ * finished beam has the one candidate (i, eos_token) with scores[i].  The n best go to
+ * tokens, parents [B, n] int32 and new_scores [B, n] fp32, best first.  Candidates of one
+ * beam are ordered by logit, equal ones by token; beams are merged by score in 64 bits,
+ * equal ones by beam.  Candidates without a finite score (masked tokens at -inf, beams with
+ * scores[i] = -inf, rows that hold a NaN or +inf) are never chosen; places left over get
+ * token -1, parent -1, score -inf.  K <= 64, n <= 64 (GDN_ERR_LIMIT).
+ */
+GDN_API size_t gdn_beam_select_workspace_bytes(int B, int K, int V, int n);
+GDN_API int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch,
+                            int64_t stride_beam, const float* scores,
+                            const uint8_t* finished, int eos_token, int B, int K, int V,
+                            int n, int32_t* tokens, int32_t* parents, float* new_scores,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Pages of a cache: slots of a pooled state, pages of a key-value cache.
+ *
+ * A pool is num_pages pages of page_bytes[i] bytes, page_pitch[i] bytes apart; up to 32
+ * pools (layers, keys and values) that share one page numbering go through one call.
+ * Pools may interleave but not share a byte (GDN_ERR_ALIAS).  refcounts [num_pages] int32:
+ * a page is free when its count is <= 0.
+ *
+ * gdn_copy_pages: pools[dst[i]] = pools[src[i]] for i < n (<= 4096) as one simultaneous
+ * assignment: sources are read as they were before the call, also where they are
+ * destinations; of equal dst the last valid pair wins.  A negative index skips its pair, one
+ * >= num_pages skips it and is counted in *bad_index_count (int32, may be NULL).
+ */
+GDN_API int gdn_copy_pages(void* const* pools, const int64_t* page_bytes,
+                           const int64_t* page_pitch, int num_pools, int num_pages,
+                           const int32_t* src, const int32_t* dst, int n,
+                           int32_t* bad_index_count, void* stream);
+
+/*
+ * pages[i] = the next lowest free page (its count becomes 1) for each i with need[i] != 0,
+ * in order of i; -1 where need[i] == 0 or no page is left.  workspace: 4 n bytes.
+ */
+GDN_API int gdn_alloc_pages(int32_t* refcounts, int num_pages, const uint8_t* need, int n,
+                            int32_t* pages, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/*
+ * One reference less for every entry of pages [n]; negative entries are skipped.  An entry
+ * >= num_pages and one whose page has no reference left are counted in *bad_index_count.
+ */
+GDN_API int gdn_free_pages(int32_t* refcounts, int num_pages, const int32_t* pages, int64_t n,
+                           int32_t* bad_index_count, void* stream);
+
+/*
+ * Forks sequences of a paged cache: row i of new_tables [rows_out, table_width] and
+ * new_lens is a child of row parents[i] of block_tables [rows_in, table_width] (row stride
+ * table_stride) and seq_lens.  With c children of a row, each of its full pages gets c - 1
+ * references more (so a row without children gives its pages up); its partly filled last
+ * page stays with its first child, and every other child gets the lowest free page left
+ * (after those changes; in order of i) as a copy of it in all pools.  Entries behind a row's
+ * tokens are -1.  parents[i] outside [0, rows_in) makes an empty row (>= rows_in is counted
+ * in *bad_index_count).  Where no page is left for a copy the entry is -1 and is counted.
+ * A partly filled last page must have no reference but its row's.  workspace: 12 rows_out
+ * bytes.  new_tables and new_lens may not overlap their inputs.
+ */
+GDN_API int gdn_fork_pages(const int32_t* block_tables, int64_t table_stride,
+                           const int32_t* seq_lens, const int32_t* parents,
+                           int32_t* refcounts, int32_t* new_tables, int32_t* new_lens,
+                           int rows_in, int rows_out, int table_width, int num_pages,
+                           int page_size, void* const* pools, const int64_t* page_bytes,
+                           const int64_t* page_pitch, int num_pools, void* workspace,
+                           size_t workspace_bytes, int32_t* bad_index_count, void* stream);
+
+/*
+ * Moves the live pages into the first num_live ones: the k-th live page at or behind
+ * num_live (ascending) takes the k-th free page before it, with its reference count, in all
+ * pools.  remap [num_pages] gets each live page's new number, -1 for a free one;
+ * block_tables (table_entries int32 in a row, may be NULL with 0) is rewritten through it in
+ * place, entries outside [0, num_pages) stay.  workspace: 4 (2 (num_pages / 2 + 1) + 1) bytes.
+ */
+GDN_API int gdn_compact_pages(int32_t* refcounts, int num_pages, int32_t* block_tables,
+                              int64_t table_entries, int32_t* remap, int32_t* num_live,
+                              void* const* pools, const int64_t* page_bytes,
+                              const int64_t* page_pitch, int num_pools, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
