@@ -14,6 +14,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "serving_common.cuh"
 
 namespace {
@@ -31,10 +33,13 @@ struct AttnArgs {
   void* out;                 // [B, HQ, D]
   float* lse;                // [B, HQ] or null
   int32_t* bad;              // or null
+  float* part_o;             // workspace [2 grid, heads of a row, D]: sums of p v
+  float* part_ml;            // workspace [2 grid, heads of a row, 2]: their m and l
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // byte strides
   long long table_stride;
   float scale_log2;          // scale * log2(e): the softmax runs in base 2
-  int B, HQ, HKV, group, num_pages, page_size, width, window, sinks;
+  uint32_t page_mul, page_shift;
+  int B, HQ, HKV, group, tiles, grid, num_pages, page_size, width, window, sinks;
 };
 
 // One sequence's lengths: tokens held, tokens visible, whether the new token is in play.
@@ -55,94 +60,549 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& p, int b) {
   return s;
 }
 
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+// ------------------------------------------------------------------ split of the work
+//
+// A "row" is (sequence, key-value head, tile of 8 or 16 of its query heads); it has
+// ceil(vis / kBlock) blocks of tokens, at least one.  All rows' blocks in a line are cut
+// into equal shares, one per CTA, so ragged batches, one long sequence and many short ones
+// all load the GPU evenly.  A CTA that has all of a row writes its output; a row that is
+// cut leaves partial sums (at most two per CTA: its first and its last row), which
+// attn_join_kernel adds up in a fixed order.  The cut depends on lens alone, so no
+// counters or flags are kept in memory.
+
+constexpr int kWarps = 4;
+constexpr int kTile = 16;                // tokens a warp takes at a time
+constexpr int kBlock = kWarps * kTile;
+
+__device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
+  const int vis = sequence(p, b).vis;
+  return vis > 0 ? (vis + kBlock - 1) / kBlock : 1;
+}
+
+// CTAs that get a share of n blocks: each at least one block.
+__device__ __forceinline__ long long shares(const AttnArgs& p, long long n) {
+  return n < p.grid ? n : p.grid;
+}
+// the share that block i lies in, and the first block of share c
+__device__ __forceinline__ long long share_of(long long i, long long n, long long g) {
+  return ((i + 1) * g - 1) / n;
+}
+__device__ __forceinline__ long long share_start(long long c, long long n, long long g) {
+  return c * n / g;
+}
+
+// Sums over the sequences, by all threads of a CTA of N threads: blocks of all of them and
+// of those before `b`.
+template <int N>
+__device__ void count_blocks(const AttnArgs& p, int b, long long& all, long long& before) {
+  __shared__ long long sa[N / 32], sb[N / 32];
+  long long x = 0, y = 0;
+  for (int i = threadIdx.x; i < p.B; i += N) {
+    const int n = blocks_of(p, i);
+    x += n;
+    y += i < b ? n : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    y += __shfl_xor_sync(0xffffffffu, y, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sa[threadIdx.x / 32] = x;
+    sb[threadIdx.x / 32] = y;
+  }
+  __syncthreads();
+  all = before = 0;
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) {
+    all += sa[i];
+    before += sb[i];
+  }
+}
+
+// The sequence that holds block `at` of a key-value head row's line (at < all sequences'
+// blocks), and the blocks before it.  By all threads of the CTA.
+__device__ void find_sequence(const AttnArgs& p, long long at, int& b, long long& before) {
+  __shared__ long long sum[kWarps], found_before;
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  long long base = 0;
+  if (tid == 0) found = -1;
+  for (int b0 = 0;; b0 += kWarps * 32) {
+    const int n = b0 + tid < p.B ? blocks_of(p, b0 + tid) : 0;
+    long long x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();                     // the last round's readers of sum are done
+    if (lane == 31) sum[warp] = x;
+    __syncthreads();
+    long long total = 0, mine = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mine += w < warp ? sum[w] : 0;
+      total += sum[w];
+    }
+    const long long first = base + mine + x - n;
+    if (n > 0 && first <= at && at < first + n) {
+      found = b0 + tid;
+      found_before = first;
+    }
+    base += total;
+    __syncthreads();
+    if (found >= 0 || b0 + kWarps * 32 >= p.B) break;
+  }
+  b = found;
+  before = found_before;
+}
+
+// ------------------------------------------------------------------ matrix instructions
+
 template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16(x); }
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half(x); }
 
-// One CTA of 4 warps per (query head, sequence); warp w takes tokens w, w+4, ...; lane j
-// holds dims j, j+32, ...
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_decode_kernel(AttnArgs p) {
-  constexpr int N = D / 32;
-  const int h = blockIdx.x, b = blockIdx.y, g = h / p.group;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const Seq s = sequence(p, b);
-  const int32_t* table = p.tables + b * p.table_stride;
-  const T* kn = reinterpret_cast<const T*>(p.k_new) + (static_cast<long long>(b) * p.HKV + g) * D;
-  const T* vn = reinterpret_cast<const T*>(p.v_new) + (static_cast<long long>(b) * p.HKV + g) * D;
-  const T* q = reinterpret_cast<const T*>(p.q) + (static_cast<long long>(b) * p.HQ + h) * D;
-  float qf[N], o[N], m = -INFINITY, l = 0.f;
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// c[16 x 8] += a[16 x 16] b[16 x 8]
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// four 8 x 8 matrices of 16-bit values; lane l gives the address of row l % 8 of matrix l / 8
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------ the kernel
+//
+// Both products run transposed, with the tokens (then the head dims) as the 16 rows of the
+// matrix instruction and 8 query heads as its columns:
+//   S^T [16 tokens x 8 heads] = K Q^T        O^T [D x 8 heads] += V^T P^T
+// so a group of up to 8 query heads fills the instruction, where queries as rows would
+// leave half of it empty, and the accumulators of O take D / 16 x 4 registers.  The scores'
+// accumulator layout becomes the second product's operand by an 8 x 8 transpose in
+// registers.  p is rounded to the tensors' type for that product (its own sum l is not):
+// the rounding is that of the values it multiplies, at most half a step of each weight.
+//
+// Every warp streams its own 16-token tiles through its own ring of kStages buffers in
+// shared memory with asynchronous copies, so the main loop has no CTA barrier.  A tile's page
+// numbers are loaded one tile before its copies are issued.
+
+template <int D> struct Shape {
+  static constexpr int kRow = D * 2;                          // bytes of a token's row
+  static constexpr int kHalf = kTile * kRow;                  // K or V part of a stage
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kWarpBytes = kStages * 2 * kHalf;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kResident = D == 64 ? 3 : D == 128 ? 2 : 1;   // CTAs per SM
+};
+
+// 16-byte chunk c of row r in a tile, spread over the banks for the matrix loads
+template <int D> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return r * Shape<D>::kRow + ((c ^ (r & 7)) << 4);
+}
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(kWarps * 32, Shape<D>::kResident)
+attn_decode_kernel(const __grid_constant__ AttnArgs p) {
+  using S = Shape<D>;
+  constexpr int kHeads = 8 * NG, KS = D / 16, CPR = D / 8;    // chunks per row
+  constexpr int kPad = D + 4;                                 // floats of a head in the merge
+  static_assert(kHeads * kPad * 4 <= S::kWarpBytes, "the merge reuses the ring");
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
+
+  long long per_row, unused;
+  count_blocks<kWarps * 32>(p, 0, per_row, unused);
+  const int rows = p.HKV * p.tiles;                           // rows of one sequence
+  const long long total = per_row * rows, g_eff = shares(p, total);
+  if (blockIdx.x >= g_eff) return;
+  long long at = share_start(blockIdx.x, total, g_eff);
+  const long long end = share_start(blockIdx.x + 1, total, g_eff), start = at;
+  int b;
+  long long before;
+  find_sequence(p, at / rows, b, before);                     // line order: sequence, row, block
+
+  while (at < end) {
+    const Seq s = sequence(p, b);
+    const int nb = s.vis > 0 ? (s.vis + kBlock - 1) / kBlock : 1;
+    const long long in_seq = at - before * rows;
+    const int row = static_cast<int>(in_seq / nb), k0 = static_cast<int>(in_seq % nb);
+    const long long left = end - at;
+    const int k1 = left < nb - k0 ? k0 + static_cast<int>(left) : nb;
+    const int g = row / p.tiles, tile = row % p.tiles;
+    const int head0 = g * p.group + tile * kHeads, heads = min(kHeads, p.group - tile * kHeads);
+    const int32_t* table = p.tables + b * p.table_stride;
+    const long long new_row = (static_cast<long long>(b) * p.HKV + g) * D * 2;
+    const char* kbase = p.k + g * p.k_head;
+    const char* vbase = p.v + g * p.v_head;
+    const bool counts = row == 0 && p.bad != nullptr;
+    if (counts && tid == 0 && k0 == 0 && p.lens[b] > s.len) atomicAdd(p.bad, 1);
+
+    // lane i < 16 looks after token i of a tile: its page number, its place, whether it is seen
+    auto token_of = [&](int k) {
+      const int j = (k * kWarps + warp) * kTile + (lane & 15);
+      return j < s.vis ? (j < p.sinks ? j : j + s.shift) : -1;
+    };
+    auto page_of = [&](int k) {
+      const int tok = k < k1 ? token_of(k) : -1;
+      return tok < 0 ? -1 : __ldg(table + div_by(tok, p.page_mul, p.page_shift));
+    };
+    // whether no visible token before tok lies in its page
+    auto first_in_page = [&](int tok, int off) {
+      if (off == 0) return true;
+      return s.shift > 0 && tok == p.sinks + s.shift &&
+             (p.sinks == 0 || (p.sinks - 1) / p.page_size != tok / p.page_size);
+    };
+    // issue the copies of block k's tile into ring stage st; returns the tokens seen
+    auto fetch = [&](int k, int st, int page) -> uint32_t {
+      const int tok = token_of(k);
+      const int off = tok < 0 ? 0 : tok - static_cast<int>(div_by(tok, p.page_mul, p.page_shift)) * p.page_size;
+      const bool is_new = s.append && tok == s.len - 1;
+      const bool seen = tok >= 0 && (is_new || (page >= 0 && page < p.num_pages));
+      if (counts && lane < 16 && tok >= 0 && page >= p.num_pages && first_in_page(tok, off))
+        atomicAdd(p.bad, 1);
+      const uint32_t mask = __ballot_sync(0xffffffffu, seen) & 0xffffu;
+      const uint32_t news = __ballot_sync(0xffffffffu, is_new) & 0xffffu;
+      const uint32_t dst = ring + st * 2 * S::kHalf;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    qf[i] = to_f(q[lane + 32 * i]);
-    o[i] = 0.f;
-  }
-  if (h == 0 && threadIdx.x == 0 && p.bad && p.lens[b] > s.len) atomicAdd(p.bad, 1);
-  for (int j = warp; j < s.vis; j += 4) {
-    const int tok = j < p.sinks ? j : j + s.shift;
-    const int page = table[tok / p.page_size], off = tok % p.page_size;
-    const bool in_new = s.append && tok == s.len - 1;
-    const bool ok = page >= 0 && page < p.num_pages;
-    if (h == 0 && lane == 0 && p.bad && page >= p.num_pages &&
-        (off == 0 || j == 0 || (j == p.sinks && p.window > 0)))
-      atomicAdd(p.bad, 1);
-    char* krow = p.k + (ok ? page * p.k_page + off * p.k_tok + g * p.k_head : 0);
-    char* vrow = p.v + (ok ? page * p.v_page + off * p.v_tok + g * p.v_head : 0);
-    if (in_new && ok && h % p.group == 0) {
+      for (int i = 0; i < CPR / 2; ++i) {
+        const int f = lane + 32 * i, r = f / CPR, c = f % CPR;
+        const int pg = __shfl_sync(0xffffffffu, page, r), of = __shfl_sync(0xffffffffu, off, r);
+        const bool ok = (mask >> r) & 1;
+        const char* ks = kbase + pg * p.k_page + of * p.k_tok;
+        const char* vs = vbase + pg * p.v_page + of * p.v_tok;
+        if ((news >> r) & 1) {
+          ks = reinterpret_cast<const char*>(p.k_new) + new_row;
+          vs = reinterpret_cast<const char*>(p.v_new) + new_row;
+        }
+        if (!ok) {
+          ks = kbase;
+          vs = vbase;
+        }
+        copy16_async(dst + chunk_at<D>(r, c), ks + c * 16, ok);
+        copy16_async(dst + S::kHalf + chunk_at<D>(r, c), vs + c * 16, ok);
+      }
+      return mask;
+    };
+
+    uint32_t mask[S::kStages];
+    int page = page_of(k0);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        reinterpret_cast<T*>(krow)[lane + 32 * i] = kn[lane + 32 * i];
-        reinterpret_cast<T*>(vrow)[lane + 32 * i] = vn[lane + 32 * i];
+    for (int st = 0; st < S::kStages - 1; ++st) {
+      mask[st] = 0;
+      const int next = page_of(k0 + st + 1);
+      if (k0 + st < k1) mask[st] = fetch(k0 + st, st, page);
+      page = next;
+      copy_commit();
+    }
+    // the new token's rows go into the cache once: by the first tile's owner of the last block
+    if (s.append && tile == 0 && k1 == nb) {
+      const int tok = s.len - 1, pi = tok / p.page_size, pg = table[pi];
+      if (pg >= 0 && pg < p.num_pages && tid < 2 * CPR) {
+        const int c = tid % CPR, of = tok - pi * p.page_size;
+        const char* src = reinterpret_cast<const char*>(tid < CPR ? p.k_new : p.v_new) + new_row;
+        char* dst = tid < CPR ? p.k + g * p.k_head + pg * p.k_page + of * p.k_tok
+                              : p.v + g * p.v_head + pg * p.v_page + of * p.v_tok;
+        *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(src + c * 16);
       }
     }
-    if (!ok && !in_new) continue;
-    const T* kr = in_new ? kn : reinterpret_cast<const T*>(krow);
-    const T* vr = in_new ? vn : reinterpret_cast<const T*>(vrow);
-    float x = 0.f;
+    // queries as the right operand: head lane / 4 (+ 8 per further group), two dims a register
+    uint32_t qf[NG][KS][2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x += qf[i] * to_f(kr[lane + 32 * i]);
-    x = warp_sum(x) * p.scale_log2;
-    const float mn = fmaxf(m, x);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float c = exp2f(m - base), e = exp2f(x - base);
-    l = l * c + e;
+    for (int n = 0; n < NG; ++n) {
+      const int h = n * 8 + lane / 4;
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q) +
+                          (static_cast<long long>(b) * p.HQ + head0 + (h < heads ? h : 0)) * (D / 2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * c + e * to_f(vr[lane + 32 * i]);
-    m = mn;
+      for (int i = 0; i < KS; ++i) {
+        qf[n][i][0] = h < heads ? __ldg(q + i * 8 + lane % 4) : 0u;
+        qf[n][i][1] = h < heads ? __ldg(q + i * 8 + 4 + lane % 4) : 0u;
+      }
+    }
+
+    float o[NG][KS][4], m[NG][2], l[NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+    }
+
+    int st = 0;
+    for (int k = k0; k < k1; ++k) {
+      copy_wait<S::kStages - 2>();
+      __syncwarp();
+      const uint32_t buf = ring + st * 2 * S::kHalf;
+      const uint32_t seen = mask[0];
+      float x[NG][2][4];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t a[4];
+        load_matrices(a, buf + chunk_at<D>(lane % 16, 2 * i + lane / 16));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+      }
+      uint32_t pb[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
+        if (seen != 0xffffu) {
+          if (!((seen >> (lane / 4)) & 1)) y[0] = y[1] = -INFINITY;
+          if (!((seen >> (lane / 4 + 8)) & 1)) y[2] = y[3] = -INFINITY;
+        }
+        float t0 = fmaxf(y[0], y[2]), t1 = fmaxf(y[1], y[3]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+        }
+        const float m0 = fmaxf(m[n][0], t0), m1 = fmaxf(m[n][1], t1);
+        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+        if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1])) {
+          const float c0 = exp2_fast(m[n][0] - b0), c1 = exp2_fast(m[n][1] - b1);
+          l[n][0] *= c0;
+          l[n][1] *= c1;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            o[n][i][0] *= c0;
+            o[n][i][1] *= c1;
+            o[n][i][2] *= c0;
+            o[n][i][3] *= c1;
+          }
+          m[n][0] = m0;
+          m[n][1] = m1;
+        }
+        const float p0 = exp2_fast(y[0] - b0), p1 = exp2_fast(y[1] - b1);
+        const float p2 = exp2_fast(y[2] - b0), p3 = exp2_fast(y[3] - b1);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+        pb[n][0] = transpose8(pack2<T>(p0, p1));
+        pb[n][1] = transpose8(pack2<T>(p2, p3));
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t a[4];
+        load_matrices_t(a, buf + S::kHalf + chunk_at<D>((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[n][0], pb[n][1]);
+      }
+      __syncwarp();                       // every lane is done with this stage
+#pragma unroll
+      for (int i = 0; i + 1 < S::kStages - 1; ++i) mask[i] = mask[i + 1];
+      mask[S::kStages - 2] = 0;
+      const int kn = k + S::kStages - 1;
+      const int next = page_of(kn + 1);
+      if (kn < k1) mask[S::kStages - 2] = fetch(kn, st == 0 ? S::kStages - 1 : st - 1, page);
+      page = next;
+      copy_commit();
+      st = st + 1 == S::kStages ? 0 : st + 1;
+    }
+    copy_wait<0>();
+    __syncwarp();
+
+    // the four warps' sums, through shared memory (each in its own ring)
+    float* mine = reinterpret_cast<float*>(smem + warp * S::kWarpBytes);
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], d);
+        l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], d);
+      }
+      const int h = n * 8 + 2 * (lane % 4);
+      if (lane < 4) {
+        sm_m[warp][h] = m[n][0];
+        sm_m[warp][h + 1] = m[n][1];
+        sm_l[warp][h] = l[n][0];
+        sm_l[warp][h + 1] = l[n][1];
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int d = i * 16 + lane / 4;
+        mine[h * kPad + d] = o[n][i][0];
+        mine[(h + 1) * kPad + d] = o[n][i][1];
+        mine[h * kPad + d + 8] = o[n][i][2];
+        mine[(h + 1) * kPad + d + 8] = o[n][i][3];
+      }
+    }
+    __syncthreads();
+    const bool whole = k0 == 0 && k1 == nb;
+    const long long slot = 2 * static_cast<long long>(blockIdx.x) + (at == start ? 0 : 1);
+    for (int f = tid; f < heads * (D / 2); f += kWarps * 32) {
+      const int h = f / (D / 2), d = (f % (D / 2)) * 2;
+      float mx = sm_m[0][h];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][h]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float lt = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float c = exp2_fast(sm_m[w][h] - base);
+        const float* other = reinterpret_cast<const float*>(smem + w * S::kWarpBytes) + h * kPad + d;
+        lt += sm_l[w][h] * c;
+        a0 += other[0] * c;
+        a1 += other[1] * c;
+      }
+      if (whole) {
+        const long long r = static_cast<long long>(b) * p.HQ + head0 + h;
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        reinterpret_cast<uint32_t*>(p.out)[(r * D + d) / 2] = pack2<T>(a0 * inv, a1 * inv);
+        if (d == 0 && p.lse) p.lse[r] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+      } else {
+        *reinterpret_cast<float2*>(p.part_o + (slot * kHeads + h) * D + d) = make_float2(a0, a1);
+        if (d == 0)
+          *reinterpret_cast<float2*>(p.part_ml + (slot * kHeads + h) * 2) = make_float2(mx, lt);
+      }
+    }
+    __syncthreads();                      // the ring is free for the next row
+    at += k1 - k0;
+    if (row == rows - 1 && k1 == nb) {
+      before += nb;
+      ++b;
+    }
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+  grid_trigger();
+}
+
+// Adds up the parts of a row that was cut: o = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+// One CTA per (query head, sequence); rows that were not cut are left alone.
+constexpr int kJoinThreads = 256;
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnArgs p) {
+  constexpr int kHeads = 8 * NG, kPer = kJoinThreads / D;     // parts side by side
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int g = h / p.group, hh = h % p.group, tile = hh / kHeads, col = hh % kHeads;
+  __shared__ float weight[3 * kSMs + 2], acc[kJoinThreads], red[kJoinThreads / 32];
+  long long per_row, before;
+  count_blocks<kJoinThreads>(p, b, per_row, before);
+  const int rows = p.HKV * p.tiles, nb = blocks_of(p, b);
+  const long long total = per_row * rows, g_eff = shares(p, total);
+  const long long first = before * rows + static_cast<long long>(g * p.tiles + tile) * nb;
+  const int c0 = static_cast<int>(share_of(first, total, g_eff));
+  const int c1 = static_cast<int>(share_of(first + nb - 1, total, g_eff));
+  grid_wait();                            // also where nothing is joined: the call ends after both
+  if (c0 == c1) return;
+  const int parts = c1 - c0 + 1;
+  auto slot = [&](int i) {
+    return 2 * static_cast<long long>(c0 + i) + (i == 0 && first > share_start(c0, total, g_eff) ? 1 : 0);
+  };
+  float mx = -INFINITY;
+  for (int i = tid; i < parts; i += kJoinThreads) {
+    const float m = p.part_ml[(slot(i) * kHeads + col) * 2];
+    weight[i] = m;
+    mx = fmaxf(mx, m);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) so[warp][lane + 32 * i] = o[i];
+  mx = warp_max(mx);
+  if (tid % 32 == 0) red[tid / 32] = mx;
   __syncthreads();
-  float mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  mx = red[0];
+#pragma unroll
+  for (int i = 1; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
   const float base = mx == -INFINITY ? 0.f : mx;
+  __syncthreads();
   float lt = 0.f;
-  for (int w = 0; w < 4; ++w) lt += sl[w] * exp2f(sm[w] - base);
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float acc = 0.f;
-    for (int w = 0; w < 4; ++w) acc += so[w][d] * exp2f(sm[w] - base);
-    reinterpret_cast<T*>(p.out)[(static_cast<long long>(b) * p.HQ + h) * D + d] =
-        from_f<T>(lt == 0.f ? 0.f : acc / lt);
+  for (int i = tid; i < parts; i += kJoinThreads) {
+    const float w = exp2_fast(weight[i] - base);
+    weight[i] = w;
+    lt += w * p.part_ml[(slot(i) * kHeads + col) * 2 + 1];
   }
-  if (threadIdx.x == 0 && p.lse)
-    p.lse[static_cast<long long>(b) * p.HQ + h] =
-        lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+  lt = warp_sum(lt);
+  if (tid % 32 == 0) red[tid / 32] = lt;
+  __syncthreads();
+  lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) lt += red[i];
+  const int d = tid % D;
+  float a = 0.f;
+#pragma unroll 4
+  for (int i = tid / D; i < parts; i += kPer) a += weight[i] * p.part_o[(slot(i) * kHeads + col) * D + d];
+  acc[tid] = a;
+  __syncthreads();
+  if (tid < D) {
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) a += acc[tid + i * D];
+    const long long r = static_cast<long long>(b) * p.HQ + h;
+    reinterpret_cast<T*>(p.out)[r * D + d] = from_f<T>(lt == 0.f ? 0.f : a / lt);
+    if (tid == 0 && p.lse) p.lse[r] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+// heads of a row: one group of 8 columns, or two for larger groups of query heads
+int heads_of(int group) { return group <= 8 ? 8 : 16; }
+
+int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
+
+// CTAs of a call: what the GPU holds at once, or one per block of tokens if there are fewer
+long long grid_of(int B, int HQ, int HKV, int D, long long max_tokens) {
+  const int heads = heads_of(HQ / HKV);
+  const long long rows = static_cast<long long>(B) * HKV * ((HQ / HKV + heads - 1) / heads);
+  const long long nb = max_tokens > 0 ? (max_tokens + kBlock - 1) / kBlock : 1;
+  const long long most = static_cast<long long>(kSMs) * resident(D);
+  return rows * nb < most ? rows * nb : most;
+}
+
+template <typename T, int D, int NG>
+cudaError_t launch_shape(const AttnArgs& p, bool split, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<T, D, NG>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  attn_decode_kernel<T, D, NG><<<p.grid, kWarps * 32, Shape<D>::kSmem, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !split) return e;
+  return launch_after(attn_join_kernel<T, D, NG>, dim3(p.HQ, p.B), dim3(kJoinThreads), 0, st, p);
 }
 
 template <typename T>
-cudaError_t launch(const AttnArgs& p, int D, cudaStream_t st) {
-  const dim3 grid(p.HQ, p.B);
-  if (D == 64) attn_decode_kernel<T, 64><<<grid, 128, 0, st>>>(p);
-  else if (D == 128) attn_decode_kernel<T, 128><<<grid, 128, 0, st>>>(p);
-  else attn_decode_kernel<T, 256><<<grid, 128, 0, st>>>(p);
-  return cudaGetLastError();
+cudaError_t launch(const AttnArgs& p, int D, bool split, cudaStream_t st) {
+  const bool wide = p.group > 8;
+  if (D == 64) return wide ? launch_shape<T, 64, 2>(p, split, st) : launch_shape<T, 64, 1>(p, split, st);
+  if (D == 128) return wide ? launch_shape<T, 128, 2>(p, split, st) : launch_shape<T, 128, 1>(p, split, st);
+  return wide ? launch_shape<T, 256, 2>(p, split, st) : launch_shape<T, 256, 1>(p, split, st);
 }
 
 }  // namespace
@@ -150,8 +610,9 @@ cudaError_t launch(const AttnArgs& p, int D, cudaStream_t st) {
 extern "C" {
 
 size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D, int max_tokens) {
-  (void)B; (void)HQ; (void)HKV; (void)D; (void)max_tokens;
-  return 0;
+  if (B < 1 || HQ < 1 || HKV < 1 || HQ % HKV != 0 || (D != 64 && D != 128 && D != 256)) return 0;
+  if (max_tokens <= kBlock) return 0;    // no row is ever cut
+  return static_cast<size_t>(2 * grid_of(B, HQ, HKV, D, max_tokens)) * heads_of(HQ / HKV) * (D + 2) * 4;
 }
 
 int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
@@ -183,6 +644,11 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] % 8 || v_strides[i] % 8)
       return GDN_ERR_ALIGN;
+  const int max_tokens = table_width * page_size;
+  const size_t need = gdn_paged_attention_workspace_bytes(B, HQ, HKV, D, max_tokens);
+  if (need > 0 && !workspace) return GDN_ERR_NULL;
+  if (!aligned(workspace, 16)) return GDN_ERR_ALIGN;
+  if (workspace_bytes < need) return GDN_ERR_SHAPE;
   AttnArgs p{};
   p.q = q; p.k = static_cast<char*>(k_cache); p.v = static_cast<char*>(v_cache);
   p.tables = block_tables; p.lens = seq_lens; p.k_new = k_new; p.v_new = v_new;
@@ -195,9 +661,13 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   p.B = B; p.HQ = HQ; p.HKV = HKV; p.group = HQ / HKV; p.num_pages = num_pages;
   p.page_size = page_size; p.width = table_width; p.window = window;
   p.sinks = window > 0 ? num_sinks : 0;
-  (void)workspace; (void)workspace_bytes;
+  p.tiles = (p.group + heads_of(p.group) - 1) / heads_of(p.group);
+  p.grid = static_cast<int>(grid_of(B, HQ, HKV, D, max_tokens));
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + static_cast<size_t>(2 * p.grid) * heads_of(p.group) * D;
+  div_constants(static_cast<uint32_t>(page_size), p.page_mul, p.page_shift);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, st) : launch<__half>(p, D, st);
+  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, need > 0, st) : launch<__half>(p, D, need > 0, st);
   return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 

@@ -31,4 +31,58 @@ __device__ __forceinline__ float warp_max(float x) {
   return x;
 }
 
+constexpr int kSMs = 148;
+
+// x / d for 32-bit x by multiplication with mul and shift from div_constants
+__device__ __forceinline__ uint32_t div_by(uint32_t x, uint32_t mul, uint32_t shift) {
+  return static_cast<uint32_t>((static_cast<unsigned long long>(__umulhi(x, mul)) + x) >> shift);
+}
+inline void div_constants(uint32_t d, uint32_t& mul, uint32_t& shift) {
+  shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+}
+
+// programmatic dependent launch: a kernel waits for the one before it, or lets the next start
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Launches `kernel` as a programmatic dependent of the kernel before it on the stream; it
+// must grid_wait() before it reads anything of that kernel's.
+template <typename... Args>
+cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                         const Args&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// 16 bytes to shared memory without a register detour; zeros when !valid (src is not read)
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2^-22 relative, exp2(-inf) = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 }  // namespace gdn_serving

@@ -139,6 +139,16 @@ def test_table_entries_out_of_range_hide_their_tokens():
     assert int(bad) == want[-1]
 
 
+@pytest.mark.parametrize("sinks,window", [(0, 20), (3, 20), (17, 20), (3, 500)])
+def test_bad_pages_are_counted_once_with_a_window(sinks, window):
+    x = make([100, 30, 90], 8, 2, 64, 16)
+    x["block_tables"][:, ::2] = 1000
+    want = expect(x, window, sinks)
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(x, run(x, window=window, num_sinks=sinks, bad_index_count=bad), want)
+    assert int(bad) == want[-1]
+
+
 def test_lengths_beyond_the_table_and_negative():
     x = make([40, -3, 10], 8, 2, 128, 16, width=3)
     x["seq_lens"][0] = 49
