@@ -22,9 +22,10 @@ using namespace gdn_serving;
 
 constexpr int kMaxBeams = 64, kMaxSelected = 64;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kVecs = 16;        // 16-byte vectors of logits a thread holds at most
+constexpr int kSlice = 3072;     // 16-byte vectors of logits a CTA holds: 48 KB, four CTAs per SM
 constexpr int kList = 512;       // candidates of a slice that are ranked
 constexpr int kMergeThreads = 512;
+constexpr int kHeadItems = 1024; // of the merge's bound
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BeamArgs {
@@ -60,7 +61,7 @@ __device__ __forceinline__ int key_token(unsigned long long k) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
 }
 
-// A 16-byte vector of logits: its values, and its largest (NaNs do not count).
+// A 16-byte vector of logits.
 template <typename T> struct Vec {
   static constexpr int kN = 16 / sizeof(T);
   uint4 u;
@@ -74,6 +75,7 @@ template <typename T> struct Vec {
       return __half2float(__ushort_as_half(static_cast<unsigned short>(i % 2 ? w >> 16 : w)));
     }
   }
+  // its largest value; NaNs do not count
   __device__ __forceinline__ float largest() const {
     if constexpr (std::is_same_v<T, float>) {
       return fmaxf(fmaxf(get(0), get(1)), fmaxf(get(2), get(3)));
@@ -91,10 +93,15 @@ template <typename T> struct Vec {
 
 // ------------------------------------------------------------------ one slice of a row
 //
-// A CTA holds its slice of a row in registers: all loads are in flight at once, and the
-// slice is read once for the maximum, the sum of exponentials and the n best.  The n-th
-// largest of the threads' maxima, T, is a lower bound of the slice's n-th best; what is
-// >= T, rarely more than a few n values, is gathered in shared memory and ranked there.
+// A CTA copies its slice of a row to shared memory, all copies in flight at once; from there
+// it takes the maximum, then the sum of exponentials and the n best, so the logits cross HBM
+// once.  The n-th largest of the threads' maxima, T, is a lower bound of the slice's n-th
+// best; what is >= T, rarely more than a few n values, is gathered and ranked.
+//
+// Bound: HBM for fp32; for 16-bit logits the exponentials come near it (12.3 logits a clock
+// and SM at the measured copy rate, of 16 exponentials), so an element costs one unpack,
+// one fused multiply-add, one exponential, one addition and 1/8 of a packed maximum,
+// compare and two 16-byte loads.
 
 struct SliceShared {
   unsigned long long list[kList];
@@ -132,10 +139,12 @@ __device__ void write_ranked(const unsigned long long* list, int c, int n, unsig
   for (int i = c + threadIdx.x; i < n; i += kThreads) out[i] = 0;
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kThreads, NV > 8 ? 2 : 4) beam_slice_kernel(const BeamArgs p) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs p) {
   using V = Vec<T>;
   constexpr int E = V::kN;
+  extern __shared__ __align__(16) unsigned char smem[];
+  V* held = reinterpret_cast<V*>(smem);
   __shared__ SliceShared sh;
   const int slice = blockIdx.x % p.slices, row = blockIdx.x / p.slices, b = row / p.K, i = row % p.K;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -150,31 +159,29 @@ __global__ void __launch_bounds__(kThreads, NV > 8 ? 2 : 4) beam_slice_kernel(co
   const int v0 = static_cast<int>(static_cast<long long>(vecs) * slice / p.slices);
   const int v1 = static_cast<int>(static_cast<long long>(vecs) * (slice + 1) / p.slices);
   const uint4* base = reinterpret_cast<const uint4*>(x - mis);
-  V v[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = v0 + k * kThreads + tid;
-    const int t0 = c * E - mis;
-    if (c < v1 && t0 >= 0 && t0 + E <= p.V) {
-      v[k].u = __ldcs(base + c);
+  const int nv = v1 - v0;
+  for (int c = tid; c < nv; c += kThreads) {
+    const int t0 = (v0 + c) * E - mis;
+    if (t0 >= 0 && t0 + E <= p.V) {
+      copy16_async(smem_addr(held + c), base + v0 + c, true);
     } else {
-      T tmp[E];
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        tmp[e] = (c < v1 && t0 + e >= 0 && t0 + e < p.V) ? x[t0 + e] : T(-INFINITY);
-      v[k].u = *reinterpret_cast<uint4*>(tmp);
+        reinterpret_cast<T*>(held + c)[e] = (t0 + e >= 0 && t0 + e < p.V) ? x[t0 + e] : T(-INFINITY);
     }
   }
-  float m = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) m = fmaxf(m, v[k].largest());
-  const float mine = sort_lanes(m, lane);
-  sh.lane_max[tid] = mine;
-  if (lane == 0) sh.red[warp] = mine;
+  copy_commit();
   if (tid == 0) {
     sh.count = 0;
     sh.bound = -INFINITY;
   }
+  copy_wait<0>();                // a thread looks at its own vectors only: no barrier
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int c = tid; c < nv; c += kThreads) m = fmaxf(m, held[c].largest());
+  const float mine = sort_lanes(m, lane);
+  sh.lane_max[tid] = mine;
+  if (lane == 0) sh.red[warp] = mine;
   __syncthreads();
   m = sh.red[0];
 #pragma unroll
@@ -185,29 +192,45 @@ __global__ void __launch_bounds__(kThreads, NV > 8 ? 2 : 4) beam_slice_kernel(co
   if (lane < p.n) {
     int rank = lane;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) continue;
+    for (int o = 1; o < kWarps; ++o) {
+      const int w = (warp + o) % kWarps;
+      const float* other = sh.lane_max + w * 32;
       int lo = 0;
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1) {
-        const float y = sh.lane_max[w * 32 + lo + s - 1];
+        const float y = other[lo + s - 1];
         if (w < warp ? y >= mine : y > mine) lo += s;
       }
-      {
-        const float y = sh.lane_max[w * 32 + lo];
-        if (w < warp ? y >= mine : y > mine) ++lo;
-      }
-      rank += lo;
+      const float y = other[lo];
+      rank += lo + (w < warp ? y >= mine : y > mine);
     }
     if (rank == p.n - 1) sh.bound = mine;
   }
-  // sum of exp(x - m): x - m is rounded once, the factor log2 e once more; four chains
+  __syncthreads();
+  // sum of 2^(x f - c) with f = log2 e and c = m f as rounded; what the rounding of c took is
+  // put back once at the end.  Four chains of additions per thread.  Where m f could
+  // overflow (a slice masked with the type's lowest value) two different logits are so far
+  // apart that any small f gives the same sum.
+  const float base_m = isfinite(m) ? m : 0.f, f = fabsf(base_m) < 1e30f ? kLog2e : 0x1p-64f;
+  const float c0 = base_m * f;
+  const float bound = sh.bound;
   float s4[4] = {0.f, 0.f, 0.f, 0.f};
-  const float base_m = isfinite(m) ? m : 0.f;
+#pragma unroll 2
+  for (int c = tid; c < nv; c += kThreads) {
+    const V v = held[c];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int e = 0; e < E; ++e) s4[e % 4] += exp2_fast((v[k].get(e) - base_m) * kLog2e);
+    for (int e = 0; e < E; ++e) s4[e % 4] += exp2_fast(fmaf(v.get(e), f, -c0));
+    if (v.largest() >= bound) {
+      const int t0 = (v0 + c) * E - mis;
+      for (int e = 0; e < E; ++e) {
+        const float y = to_f(reinterpret_cast<const T*>(held + c)[e]);
+        if (y >= bound && y > -INFINITY) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kList) sh.list[at] = make_key(y, t0 + e);
+        }
+      }
+    }
+  }
   double s = static_cast<double>(s4[0] + s4[1]) + static_cast<double>(s4[2] + s4[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -217,24 +240,9 @@ __global__ void __launch_bounds__(kThreads, NV > 8 ? 2 : 4) beam_slice_kernel(co
     s = sh.sum[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) s += sh.sum[w];
+    s *= static_cast<double>(exp2f(-fmaf(base_m, f, -c0)));
     p.sums[static_cast<long long>(row) * p.slices + slice] = make_float2(m, static_cast<float>(s));
   }
-  // gather what is at or above the bound
-  const float bound = sh.bound;
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (v[k].largest() >= bound) {
-      const int t0 = (v0 + k * kThreads + tid) * E - mis;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float y = v[k].get(e);
-        if (y >= bound && y > -INFINITY) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kList) sh.list[at] = make_key(y, t0 + e);
-        }
-      }
-    }
-  __syncthreads();
   if (sh.count <= kList) {
     write_ranked(sh.list, sh.count, p.n, out);
     return;
@@ -302,8 +310,9 @@ __global__ void __launch_bounds__(kThreads, NV > 8 ? 2 : 4) beam_slice_kernel(co
 
 // ------------------------------------------------------------------ the merge
 //
-// One CTA per request.  A candidate's rank among its beam's slices, then among all beams,
-// is counted by binary searches in the sorted lists; whoever has a rank below n writes
+// One CTA per request.  The n-th best of the slices' first candidates is a lower bound of the
+// result's n-th best.  What reaches it gets its rank, among its beam's slices and then among
+// all beams, by binary searches in the sorted lists; whoever has a rank below n writes
 // itself to that place, so nothing depends on the order in which threads run.
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArgs p) {
@@ -312,10 +321,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
   int* token = reinterpret_cast<int*>(score + p.K * p.n);            // [K, n]
   double* lse = reinterpret_cast<double*>(token + p.K * p.n + (p.K * p.n & 1));   // [K]
   __shared__ int alive;
+  __shared__ double head[kHeadItems], bound;
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int per_beam = p.slices * p.n;
   for (int f = tid; f < p.K * p.n; f += kMergeThreads) score[f] = -INFINITY;
-  if (tid == 0) alive = 0;
+  if (tid == 0) {
+    alive = 0;
+    bound = -INFINITY;
+  }
   grid_wait();
   for (int i = warp; i < p.K; i += kMergeThreads / 32) {
     const int row = b * p.K + i;
@@ -338,14 +351,38 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
     if (lane == 0) lse[i] = l;          // not finite: a row that holds no candidate
   }
   __syncthreads();
-  // each beam's n best of its slices
+  // the first `depth` candidates of every slice (of as many slices as fit), at least n where
+  // there are as many
+  const unsigned long long* all = p.keys + static_cast<long long>(b) * p.K * per_beam;
+  const int lists = p.K * p.slices, depth = (p.n + lists - 1) / lists;
+  const int items = min(lists * depth, kHeadItems);
+  for (int f = tid; f < items; f += kMergeThreads) {
+    const int list = f % lists, i = list / p.slices, r = f / lists;
+    double sc = -INFINITY;
+    if (isfinite(lse[i])) {
+      const unsigned long long k = all[list * p.n + r];
+      if (k) sc = static_cast<double>(p.scores[b * p.K + i]) + (static_cast<double>(key_logit(k)) - lse[i]);
+    }
+    head[f] = sc;
+  }
+  __syncthreads();
+  for (int f = tid; f < items; f += kMergeThreads) {
+    const double sc = head[f];
+    int rank = 0;
+    for (int o = 0; o < items; ++o) rank += head[o] > sc || (head[o] == sc && o < f);
+    if (rank == p.n - 1) bound = sc;
+  }
+  __syncthreads();
+  // each beam's candidates at or above the bound, in order
   for (int f = tid; f < p.K * per_beam; f += kMergeThreads) {
     const int i = f / per_beam, at = f % per_beam, s = at / p.n, r = at % p.n;
     if (!isfinite(lse[i])) continue;
-    const unsigned long long* keys =
-        p.keys + (static_cast<long long>(b) * p.K + i) * per_beam;
+    const unsigned long long* keys = all + i * per_beam;
     const unsigned long long k = keys[at];
     if (k == 0) continue;
+    const double sc =
+        static_cast<double>(p.scores[b * p.K + i]) + (static_cast<double>(key_logit(k)) - lse[i]);
+    if (!(sc >= bound)) continue;
     int rank = r;
     for (int o = 0; o < p.slices && rank < p.n; ++o) {
       if (o == s) continue;
@@ -358,8 +395,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
       rank += lo;
     }
     if (rank < p.n) {
-      score[i * p.n + rank] =
-          static_cast<double>(p.scores[b * p.K + i]) + (static_cast<double>(key_logit(k)) - lse[i]);
+      score[i * p.n + rank] = sc;
       token[i * p.n + rank] = key_token(k);
     }
   }
@@ -407,28 +443,27 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
 
 // ------------------------------------------------------------------ host
 
-// Slices of a row of 16-byte vectors with `per` logits: as few as the registers of a CTA
-// hold, more while the rows alone do not give every SM two CTAs and a slice keeps a vector
-// for each of its threads.
+// Slices of a row of 16-byte vectors with `per` logits: as few as a CTA holds, more while
+// the rows alone do not give every SM two CTAs and a slice keeps a vector for each thread.
 int slices_of(long long rows, int V, int per) {
-  const int vecs = V / per + 2;
-  int s = (vecs + kThreads * kVecs - 1) / (kThreads * kVecs);
+  const int vecs = V / per + 2;              // of an unaligned row
+  int s = (vecs + kSlice - 1) / kSlice;
   while (rows * s < 2 * kSMs && vecs / (2 * s) >= kThreads) s *= 2;
   return s;
 }
 
 template <typename T>
 int launch(const BeamArgs& p, cudaStream_t st) {
-  const int vecs = p.V / Vec<T>::kN + 2;   // of an unaligned row
-  const int each = (vecs / p.slices + 1 + kThreads - 1) / kThreads;   // vectors a thread holds
-  const dim3 grid(p.slices * p.B * p.K);
-  if (each <= 1) beam_slice_kernel<T, 1><<<grid, kThreads, 0, st>>>(p);
-  else if (each <= 4) beam_slice_kernel<T, 4><<<grid, kThreads, 0, st>>>(p);
-  else if (each <= 8) beam_slice_kernel<T, 8><<<grid, kThreads, 0, st>>>(p);
-  else beam_slice_kernel<T, kVecs + 1><<<grid, kThreads, 0, st>>>(p);
+  const int vecs = p.V / Vec<T>::kN + 2;
+  const size_t held = static_cast<size_t>(vecs / p.slices + 1) * 16;   // of the largest slice
+  if (held > 40 * 1024 &&
+      cudaFuncSetAttribute(beam_slice_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (kSlice + 1) * 16) != cudaSuccess)
+    return GDN_ERR_LAUNCH;
+  beam_slice_kernel<T><<<p.slices * p.B * p.K, kThreads, held, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
   const size_t smem = static_cast<size_t>(p.K) * (p.n * 12 + 8) + 8;
-  if (smem > 48 * 1024 &&
+  if (smem > 32 * 1024 &&
       cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return GDN_ERR_LAUNCH;

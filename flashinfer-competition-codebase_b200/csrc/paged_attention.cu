@@ -35,11 +35,12 @@ struct AttnArgs {
   int32_t* bad;              // or null
   float* part_o;             // workspace [2 grid, heads of a row, D]: sums of p v
   float* part_ml;            // workspace [2 grid, heads of a row, 2]: their m and l
+  int4* cut;                 // workspace [grid]: the cut row that ends in this share, or none
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // byte strides
   long long table_stride;
   float scale_log2;          // scale * log2(e): the softmax runs in base 2
   uint32_t page_mul, page_shift;
-  int B, HQ, HKV, group, tiles, grid, num_pages, page_size, width, window, sinks;
+  int B, HQ, HKV, group, tiles, grid, num_pages, page_size, width, window, sinks, twin;
 };
 
 // One sequence's lengths: tokens held, tokens visible, whether the new token is in play.
@@ -63,27 +64,33 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& p, int b) {
 // ------------------------------------------------------------------ split of the work
 //
 // A "row" is (sequence, key-value head, tile of 8 or 16 of its query heads); it has
-// ceil(vis / kBlock) blocks of tokens, at least one.  All rows' blocks in a line are cut
-// into equal shares, one per CTA, so ragged batches, one long sequence and many short ones
-// all load the GPU evenly.  A CTA that has all of a row writes its output; a row that is
-// cut leaves partial sums (at most two per CTA: its first and its last row), which
-// attn_join_kernel adds up in a fixed order.  The cut depends on lens alone, so no
-// counters or flags are kept in memory.
+// ceil(vis / block) blocks of tokens, at least one.  All rows' blocks in a line (sequence,
+// row, block) are cut into equal shares, one per CTA, so ragged batches, one long sequence
+// and many short ones all load the GPU evenly.  A CTA that has all of a row writes its
+// output; a row that is cut leaves partial sums (at most two per CTA: its first and its last
+// row), which attn_join_kernel adds up in a fixed order.  The cut depends on lens alone, so
+// no counters or flags have to be kept in memory.
 
 constexpr int kWarps = 4;
-constexpr int kTile = 16;                // tokens a warp takes at a time
-constexpr int kBlock = kWarps * kTile;
 
-__device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
+// Shapes by head dim: tokens a warp takes at a time, ring stages, CTAs per SM.
+template <int D> struct Shape {
+  static constexpr int kTile = D == 64 ? 32 : 16;
+  static constexpr int kBlock = kWarps * kTile;
+  static constexpr int kRow = D * 2;                          // bytes of a token's row
+  static constexpr int kHalf = kTile * kRow;                  // K or V part of a stage
+  static constexpr int kStages = 3;
+  static constexpr int kWarpBytes = kStages * 2 * kHalf;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kResident = D == 256 ? 1 : 2;
+};
+
+template <int kBlock> __device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
   const int vis = sequence(p, b).vis;
   return vis > 0 ? (vis + kBlock - 1) / kBlock : 1;
 }
 
-// CTAs that get a share of n blocks: each at least one block.
-__device__ __forceinline__ long long shares(const AttnArgs& p, long long n) {
-  return n < p.grid ? n : p.grid;
-}
-// the share that block i lies in, and the first block of share c
+// the share of g that block i of n lies in, and the first block of share c
 __device__ __forceinline__ long long share_of(long long i, long long n, long long g) {
   return ((i + 1) * g - 1) / n;
 }
@@ -91,45 +98,22 @@ __device__ __forceinline__ long long share_start(long long c, long long n, long 
   return c * n / g;
 }
 
-// Sums over the sequences, by all threads of a CTA of N threads: blocks of all of them and
-// of those before `b`.
-template <int N>
-__device__ void count_blocks(const AttnArgs& p, int b, long long& all, long long& before) {
-  __shared__ long long sa[N / 32], sb[N / 32];
-  long long x = 0, y = 0;
-  for (int i = threadIdx.x; i < p.B; i += N) {
-    const int n = blocks_of(p, i);
-    x += n;
-    y += i < b ? n : 0;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    x += __shfl_xor_sync(0xffffffffu, x, o);
-    y += __shfl_xor_sync(0xffffffffu, y, o);
-  }
-  if (threadIdx.x % 32 == 0) {
-    sa[threadIdx.x / 32] = x;
-    sb[threadIdx.x / 32] = y;
-  }
-  __syncthreads();
-  all = before = 0;
-#pragma unroll
-  for (int i = 0; i < N / 32; ++i) {
-    all += sa[i];
-    before += sb[i];
-  }
-}
+struct Share {
+  long long total, count, start, end;    // blocks of all rows, shares, this CTA's blocks
+  long long before;                      // blocks of one row per sequence before sequence b
+  int b;                                 // the sequence of block `start`
+};
 
-// The sequence that holds block `at` of a key-value head row's line (at < all sequences'
-// blocks), and the blocks before it.  By all threads of the CTA.
-__device__ void find_sequence(const AttnArgs& p, long long at, int& b, long long& before) {
+// This CTA's share, by all its threads; start == end where there is none.
+template <int kBlock> __device__ Share my_share(const AttnArgs& p) {
+  constexpr int N = kWarps * 32;
   __shared__ long long sum[kWarps], found_before;
   __shared__ int found;
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  long long base = 0;
-  if (tid == 0) found = -1;
-  for (int b0 = 0;; b0 += kWarps * 32) {
-    const int n = b0 + tid < p.B ? blocks_of(p, b0 + tid) : 0;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, rows = p.HKV * p.tiles;
+  long long base = 0, first = 0;
+  int n = 0;
+  auto scan = [&](int b0) {              // sequences b0 ...: n and first of b0 + tid
+    n = b0 + tid < p.B ? blocks_of<kBlock>(p, b0 + tid) : 0;
     long long x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -139,30 +123,38 @@ __device__ void find_sequence(const AttnArgs& p, long long at, int& b, long long
     __syncthreads();                     // the last round's readers of sum are done
     if (lane == 31) sum[warp] = x;
     __syncthreads();
-    long long total = 0, mine = 0;
+    first = base + x - n;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      mine += w < warp ? sum[w] : 0;
-      total += sum[w];
+      first += w < warp ? sum[w] : 0;
+      base += sum[w];
     }
-    const long long first = base + mine + x - n;
+  };
+  for (int b0 = 0; b0 < p.B; b0 += N) scan(b0);
+  Share s;
+  s.total = base * rows;
+  s.count = s.total < p.grid ? s.total : p.grid;
+  s.start = s.end = 0;
+  if (blockIdx.x >= s.count) return s;
+  s.start = share_start(blockIdx.x, s.total, s.count);
+  s.end = share_start(blockIdx.x + 1, s.total, s.count);
+  const long long at = s.start / rows;
+  if (p.B > N) base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += N) {
+    if (p.B > N) scan(b0);               // else n and first are still those of sequence tid
     if (n > 0 && first <= at && at < first + n) {
       found = b0 + tid;
       found_before = first;
     }
-    base += total;
-    __syncthreads();
-    if (found >= 0 || b0 + kWarps * 32 >= p.B) break;
+    if (p.B > N && base > at) break;     // the same for all threads
   }
-  b = found;
-  before = found_before;
+  __syncthreads();
+  s.b = found;
+  s.before = found_before;
+  return s;
 }
 
 // ------------------------------------------------------------------ matrix instructions
-
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16(x); }
-template <> __device__ __forceinline__ __half from_f(float x) { return __float2half(x); }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
@@ -219,49 +211,47 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // shared memory with asynchronous copies, so the main loop has no CTA barrier.  A tile's page
 // numbers are loaded one tile before its copies are issued.
 
-template <int D> struct Shape {
-  static constexpr int kRow = D * 2;                          // bytes of a token's row
-  static constexpr int kHalf = kTile * kRow;                  // K or V part of a stage
-  static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kWarpBytes = kStages * 2 * kHalf;
-  static constexpr int kSmem = kWarps * kWarpBytes;
-  static constexpr int kResident = D == 64 ? 3 : D == 128 ? 2 : 1;   // CTAs per SM
-};
-
-// 16-byte chunk c of row r in a tile, spread over the banks for the matrix loads
-template <int D> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  return r * Shape<D>::kRow + ((c ^ (r & 7)) << 4);
-}
+// A tile's row r has its 16-byte chunk c at r kRow + ((c ^ (r & 7)) << 4): the eight rows that a
+// matrix load touches lie in different banks.  Stages are aligned to rows, so stepping
+// along a row is one XOR on the address.
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kWarps * 32, Shape<D>::kResident)
 attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   using S = Shape<D>;
   constexpr int kHeads = 8 * NG, KS = D / 16, CPR = D / 8;    // chunks per row
+  constexpr int MT = S::kTile / 16;                           // 16-token parts of a tile
+  constexpr int kRows = 32 / CPR, kIters = S::kTile / kRows;  // rows a warp copies at a time
+  constexpr uint32_t kAll = S::kTile == 32 ? 0xffffffffu : 0xffffu;
   constexpr int kPad = D + 4;                                 // floats of a head in the merge
   static_assert(kHeads * kPad * 4 <= S::kWarpBytes, "the merge reuses the ring");
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
 
-  long long per_row, unused;
-  count_blocks<kWarps * 32>(p, 0, per_row, unused);
+  grid_trigger();                         // the join's CTAs may take their places and wait
+  const Share share = my_share<S::kBlock>(p);
   const int rows = p.HKV * p.tiles;                           // rows of one sequence
-  const long long total = per_row * rows, g_eff = shares(p, total);
-  if (blockIdx.x >= g_eff) return;
-  long long at = share_start(blockIdx.x, total, g_eff);
-  const long long end = share_start(blockIdx.x + 1, total, g_eff), start = at;
-  int b;
-  long long before;
-  find_sequence(p, at / rows, b, before);                     // line order: sequence, row, block
+  long long at = share.start, before = share.before;
+  int b = share.b;
+  if (at == share.end) {
+    if (tid == 0 && p.cut) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
 
-  while (at < end) {
+  // fixed parts of this lane's addresses
+  const int copy_r = lane / CPR, copy_c = lane % CPR;
+  const uint32_t copy_at = copy_r * S::kRow + ((copy_c ^ copy_r) << 4);
+  const uint32_t k_at = (lane % 16) * S::kRow + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * S::kRow + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+
+  while (at < share.end) {
     const Seq s = sequence(p, b);
-    const int nb = s.vis > 0 ? (s.vis + kBlock - 1) / kBlock : 1;
+    const int nb = s.vis > 0 ? (s.vis + S::kBlock - 1) / S::kBlock : 1;
     const long long in_seq = at - before * rows;
     const int row = static_cast<int>(in_seq / nb), k0 = static_cast<int>(in_seq % nb);
-    const long long left = end - at;
+    const long long left = share.end - at;
     const int k1 = left < nb - k0 ? k0 + static_cast<int>(left) : nb;
     const int g = row / p.tiles, tile = row % p.tiles;
     const int head0 = g * p.group + tile * kHeads, heads = min(kHeads, p.group - tile * kHeads);
@@ -271,10 +261,16 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     const char* vbase = p.v + g * p.v_head;
     const bool counts = row == 0 && p.bad != nullptr;
     if (counts && tid == 0 && k0 == 0 && p.lens[b] > s.len) atomicAdd(p.bad, 1);
+    if (at == share.start && tid == 0 && p.cut) {
+      const long long first = before * rows + static_cast<long long>(row) * nb;
+      const int c0 = static_cast<int>(share_of(first, share.total, share.count));
+      p.cut[blockIdx.x] = make_int4(k0 > 0 && k1 == nb ? b : -1, row, c0,
+                                    first > share_start(c0, share.total, share.count));
+    }
 
-    // lane i < 16 looks after token i of a tile: its page number, its place, whether it is seen
+    // lane i looks after token i of a tile (all 32, or twice 16): its page number, its place
     auto token_of = [&](int k) {
-      const int j = (k * kWarps + warp) * kTile + (lane & 15);
+      const int j = (k * kWarps + warp) * S::kTile + (lane & (S::kTile - 1));
       return j < s.vis ? (j < p.sinks ? j : j + s.shift) : -1;
     };
     auto page_of = [&](int k) {
@@ -292,34 +288,44 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
       const int tok = token_of(k);
       const int off = tok < 0 ? 0 : tok - static_cast<int>(div_by(tok, p.page_mul, p.page_shift)) * p.page_size;
       const bool is_new = s.append && tok == s.len - 1;
-      const bool seen = tok >= 0 && (is_new || (page >= 0 && page < p.num_pages));
-      if (counts && lane < 16 && tok >= 0 && page >= p.num_pages && first_in_page(tok, off))
+      const bool in_cache = tok >= 0 && page >= 0 && page < p.num_pages;
+      if (counts && lane < S::kTile && tok >= 0 && page >= p.num_pages && first_in_page(tok, off))
         atomicAdd(p.bad, 1);
-      const uint32_t mask = __ballot_sync(0xffffffffu, seen) & 0xffffu;
-      const uint32_t news = __ballot_sync(0xffffffffu, is_new) & 0xffffu;
-      const uint32_t dst = ring + st * 2 * S::kHalf;
+      const uint32_t mask = __ballot_sync(0xffffffffu, in_cache || is_new) & kAll;
+      const bool any_new = __any_sync(0xffffffffu, is_new);
+      // this lane's token's row, relative to the head's first row
+      long long ko = in_cache ? page * p.k_page + off * p.k_tok : 0;
+      long long vo = in_cache ? page * p.v_page + off * p.v_tok : 0;
+      if (is_new) {
+        ko = reinterpret_cast<const char*>(p.k_new) + new_row - kbase;
+        vo = reinterpret_cast<const char*>(p.v_new) + new_row - vbase;
+      }
+      const uint32_t dst = ring + st * 2 * S::kHalf + copy_at;
+      const char* kc = kbase + copy_c * 16;
+      const char* vc = vbase + copy_c * 16;
+      if (mask == kAll && p.twin && !any_new) {               // nearly always
 #pragma unroll
-      for (int i = 0; i < CPR / 2; ++i) {
-        const int f = lane + 32 * i, r = f / CPR, c = f % CPR;
-        const int pg = __shfl_sync(0xffffffffu, page, r), of = __shfl_sync(0xffffffffu, off, r);
-        const bool ok = (mask >> r) & 1;
-        const char* ks = kbase + pg * p.k_page + of * p.k_tok;
-        const char* vs = vbase + pg * p.v_page + of * p.v_tok;
-        if ((news >> r) & 1) {
-          ks = reinterpret_cast<const char*>(p.k_new) + new_row;
-          vs = reinterpret_cast<const char*>(p.v_new) + new_row;
+        for (int i = 0; i < kIters; ++i) {
+          const long long o = __shfl_sync(0xffffffffu, ko, copy_r + i * kRows);
+          const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
+          copy16_async(d, kc + o, true);
+          copy16_async(d + S::kHalf, vc + o, true);
         }
-        if (!ok) {
-          ks = kbase;
-          vs = vbase;
+      } else {
+#pragma unroll 2
+        for (int i = 0; i < kIters; ++i) {
+          const int r = copy_r + i * kRows;
+          const long long o = __shfl_sync(0xffffffffu, ko, r), w = __shfl_sync(0xffffffffu, vo, r);
+          const bool ok = (mask >> r) & 1;
+          const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
+          copy16_async(d, kc + o, ok);
+          copy16_async(d + S::kHalf, vc + w, ok);
         }
-        copy16_async(dst + chunk_at<D>(r, c), ks + c * 16, ok);
-        copy16_async(dst + S::kHalf + chunk_at<D>(r, c), vs + c * 16, ok);
       }
       return mask;
     };
 
-    uint32_t mask[S::kStages];
+    uint32_t mask[S::kStages - 1];
     int page = page_of(k0);
 #pragma unroll
     for (int st = 0; st < S::kStages - 1; ++st) {
@@ -371,29 +377,44 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
       __syncwarp();
       const uint32_t buf = ring + st * 2 * S::kHalf;
       const uint32_t seen = mask[0];
-      float x[NG][2][4];
+      float y[MT][NG][4];
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int t = 0; t < MT; ++t) {
+        float x[NG][2][4];                // two chains of products
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
+        for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        uint32_t a[4];
-        load_matrices(a, buf + chunk_at<D>(lane % 16, 2 * i + lane / 16));
+          for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+        for (int i = 0; i < KS; ++i) {
+          uint32_t a[4];
+          load_matrices(a, (buf + k_at + t * 16 * S::kRow) ^ (i * 32));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[t][n][j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
       }
-      uint32_t pb[NG][2];
+      if (seen != kAll) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            if (!((seen >> (t * 16 + lane / 4)) & 1)) y[t][n][0] = y[t][n][1] = -INFINITY;
+            if (!((seen >> (t * 16 + lane / 4 + 8)) & 1)) y[t][n][2] = y[t][n][3] = -INFINITY;
+          }
+      }
+      uint32_t pb[MT][NG][2];
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float y[4];
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
-        if (seen != 0xffffu) {
-          if (!((seen >> (lane / 4)) & 1)) y[0] = y[1] = -INFINITY;
-          if (!((seen >> (lane / 4 + 8)) & 1)) y[2] = y[3] = -INFINITY;
+        for (int t = 0; t < MT; ++t) {
+          t0 = fmaxf(t0, fmaxf(y[t][n][0], y[t][n][2]));
+          t1 = fmaxf(t1, fmaxf(y[t][n][1], y[t][n][3]));
         }
-        float t0 = fmaxf(y[0], y[2]), t1 = fmaxf(y[1], y[3]);
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
           t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
@@ -415,20 +436,25 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
           m[n][0] = m0;
           m[n][1] = m1;
         }
-        const float p0 = exp2_fast(y[0] - b0), p1 = exp2_fast(y[1] - b1);
-        const float p2 = exp2_fast(y[2] - b0), p3 = exp2_fast(y[3] - b1);
-        l[n][0] += p0 + p2;
-        l[n][1] += p1 + p3;
-        pb[n][0] = transpose8(pack2<T>(p0, p1));
-        pb[n][1] = transpose8(pack2<T>(p2, p3));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const float p0 = exp2_fast(y[t][n][0] - b0), p1 = exp2_fast(y[t][n][1] - b1);
+          const float p2 = exp2_fast(y[t][n][2] - b0), p3 = exp2_fast(y[t][n][3] - b1);
+          l[n][0] += p0 + p2;
+          l[n][1] += p1 + p3;
+          pb[t][n][0] = transpose8(pack2<T>(p0, p1));
+          pb[t][n][1] = transpose8(pack2<T>(p2, p3));
+        }
       }
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        uint32_t a[4];
-        load_matrices_t(a, buf + S::kHalf + chunk_at<D>((lane & 7) + ((lane >> 4) << 3), 2 * i + ((lane >> 3) & 1)));
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[n][0], pb[n][1]);
-      }
+        for (int t = 0; t < MT; ++t) {
+          uint32_t a[4];
+          load_matrices_t(a, (buf + S::kHalf + v_at + t * 16 * S::kRow) ^ (i * 32));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[t][n][0], pb[t][n][1]);
+        }
       __syncwarp();                       // every lane is done with this stage
 #pragma unroll
       for (int i = 0; i + 1 < S::kStages - 1; ++i) mask[i] = mask[i + 1];
@@ -470,7 +496,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     }
     __syncthreads();
     const bool whole = k0 == 0 && k1 == nb;
-    const long long slot = 2 * static_cast<long long>(blockIdx.x) + (at == start ? 0 : 1);
+    const long long slot = 2 * static_cast<long long>(blockIdx.x) + (at == share.start ? 0 : 1);
     for (int f = tid; f < heads * (D / 2); f += kWarps * 32) {
       const int h = f / (D / 2), d = (f % (D / 2)) * 2;
       float mx = sm_m[0][h];
@@ -504,70 +530,63 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
       ++b;
     }
   }
-  grid_trigger();
 }
 
-// Adds up the parts of a row that was cut: o = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-// One CTA per (query head, sequence); rows that were not cut are left alone.
-constexpr int kJoinThreads = 256;
+// Adds up the parts of the rows that were cut: o = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+// CTA (c, y): values 512 y ... of the row whose last part is share c's, if one is.  128
+// threads take four values each, two groups of them every other part.
+constexpr int kJoinThreads = 256, kJoinValues = 512, kJoinParts = 3 * kSMs;
+
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnArgs p) {
-  constexpr int kHeads = 8 * NG, kPer = kJoinThreads / D;     // parts side by side
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int g = h / p.group, hh = h % p.group, tile = hh / kHeads, col = hh % kHeads;
-  __shared__ float weight[3 * kSMs + 2], acc[kJoinThreads], red[kJoinThreads / 32];
-  long long per_row, before;
-  count_blocks<kJoinThreads>(p, b, per_row, before);
-  const int rows = p.HKV * p.tiles, nb = blocks_of(p, b);
-  const long long total = per_row * rows, g_eff = shares(p, total);
-  const long long first = before * rows + static_cast<long long>(g * p.tiles + tile) * nb;
-  const int c0 = static_cast<int>(share_of(first, total, g_eff));
-  const int c1 = static_cast<int>(share_of(first + nb - 1, total, g_eff));
-  grid_wait();                            // also where nothing is joined: the call ends after both
-  if (c0 == c1) return;
-  const int parts = c1 - c0 + 1;
-  auto slot = [&](int i) {
-    return 2 * static_cast<long long>(c0 + i) + (i == 0 && first > share_start(c0, total, g_eff) ? 1 : 0);
-  };
+  constexpr int kHeads = 8 * NG, kHere = kJoinValues / D;     // heads of a row, of this CTA
+  __shared__ float2 ml[kJoinParts][kHere];
+  __shared__ float4 acc[kJoinValues / 4];
+  __shared__ float sum[kJoinValues / 4];
+  const int tid = threadIdx.x, y = blockIdx.y;
+  grid_wait();
+  const int4 cut = p.cut[blockIdx.x];
+  if (cut.x < 0) return;
+  const int g = cut.y / p.tiles, tile = cut.y % p.tiles, parts = blockIdx.x - cut.z + 1;
+  if (y * kHere >= p.group - tile * kHeads) return;           // heads past the group's
+  auto slot = [&](int i) { return 2 * static_cast<long long>(cut.z + i) + (i == 0 ? cut.w : 0); };
+  for (int f = tid; f < parts * kHere; f += kJoinThreads)
+    ml[f / kHere][f % kHere] = reinterpret_cast<const float2*>(p.part_ml)[slot(f / kHere) * kHeads + y * kHere + f % kHere];
+  __syncthreads();
+  const int quad = tid % (kJoinValues / 4), half = tid / (kJoinValues / 4);
+  const int hc = quad * 4 / D;
   float mx = -INFINITY;
-  for (int i = tid; i < parts; i += kJoinThreads) {
-    const float m = p.part_ml[(slot(i) * kHeads + col) * 2];
-    weight[i] = m;
-    mx = fmaxf(mx, m);
-  }
-  mx = warp_max(mx);
-  if (tid % 32 == 0) red[tid / 32] = mx;
-  __syncthreads();
-  mx = red[0];
-#pragma unroll
-  for (int i = 1; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[i]);
+  for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ml[i][hc].x);
   const float base = mx == -INFINITY ? 0.f : mx;
-  __syncthreads();
-  float lt = 0.f;
-  for (int i = tid; i < parts; i += kJoinThreads) {
-    const float w = exp2_fast(weight[i] - base);
-    weight[i] = w;
-    lt += w * p.part_ml[(slot(i) * kHeads + col) * 2 + 1];
+  const float4* from = reinterpret_cast<const float4*>(p.part_o) + y * (kJoinValues / 4) + quad;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 8
+  for (int i = half; i < parts; i += 2) {
+    const float4 v = from[slot(i) * (kHeads * D / 4)];
+    const float w = exp2_fast(ml[i][hc].x - base);
+    l += w * ml[i][hc].y;
+    a.x += w * v.x;
+    a.y += w * v.y;
+    a.z += w * v.z;
+    a.w += w * v.w;
   }
-  lt = warp_sum(lt);
-  if (tid % 32 == 0) red[tid / 32] = lt;
-  __syncthreads();
-  lt = 0.f;
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) lt += red[i];
-  const int d = tid % D;
-  float a = 0.f;
-#pragma unroll 4
-  for (int i = tid / D; i < parts; i += kPer) a += weight[i] * p.part_o[(slot(i) * kHeads + col) * D + d];
-  acc[tid] = a;
-  __syncthreads();
-  if (tid < D) {
-#pragma unroll
-    for (int i = 1; i < kPer; ++i) a += acc[tid + i * D];
-    const long long r = static_cast<long long>(b) * p.HQ + h;
-    reinterpret_cast<T*>(p.out)[r * D + d] = from_f<T>(lt == 0.f ? 0.f : a / lt);
-    if (tid == 0 && p.lse) p.lse[r] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+  if (half) {
+    acc[quad] = a;
+    sum[quad] = l;
   }
+  __syncthreads();
+  const int h = tile * kHeads + y * kHere + hc;
+  if (half || h >= p.group) return;
+  const float4 v = acc[quad];
+  l += sum[quad];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const long long r = static_cast<long long>(cut.x) * p.HQ + g * p.group + h;
+  reinterpret_cast<uint2*>(p.out)[(r * D + quad * 4 % D) / 4] =
+      make_uint2(pack2<T>((a.x + v.x) * inv, (a.y + v.y) * inv),
+                 pack2<T>((a.z + v.z) * inv, (a.w + v.w) * inv));
+  if (quad * 4 % D == 0 && p.lse)
+    p.lse[r] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
@@ -575,34 +594,37 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
 // heads of a row: one group of 8 columns, or two for larger groups of query heads
 int heads_of(int group) { return group <= 8 ? 8 : 16; }
 
+// tokens of a block, CTAs per SM
+int block_of(int D) { return D == 64 ? Shape<64>::kBlock : D == 128 ? Shape<128>::kBlock : Shape<256>::kBlock; }
 int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
 
 // CTAs of a call: what the GPU holds at once, or one per block of tokens if there are fewer
 long long grid_of(int B, int HQ, int HKV, int D, long long max_tokens) {
   const int heads = heads_of(HQ / HKV);
   const long long rows = static_cast<long long>(B) * HKV * ((HQ / HKV + heads - 1) / heads);
-  const long long nb = max_tokens > 0 ? (max_tokens + kBlock - 1) / kBlock : 1;
+  const long long nb = max_tokens > 0 ? (max_tokens + block_of(D) - 1) / block_of(D) : 1;
   const long long most = static_cast<long long>(kSMs) * resident(D);
   return rows * nb < most ? rows * nb : most;
 }
 
 template <typename T, int D, int NG>
-cudaError_t launch_shape(const AttnArgs& p, bool split, cudaStream_t st) {
+cudaError_t launch_shape(const AttnArgs& p, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<T, D, NG>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   attn_decode_kernel<T, D, NG><<<p.grid, kWarps * 32, Shape<D>::kSmem, st>>>(p);
   e = cudaGetLastError();
-  if (e != cudaSuccess || !split) return e;
-  return launch_after(attn_join_kernel<T, D, NG>, dim3(p.HQ, p.B), dim3(kJoinThreads), 0, st, p);
+  if (e != cudaSuccess || !p.cut) return e;
+  return launch_after(attn_join_kernel<T, D, NG>, dim3(p.grid, 8 * NG * D / kJoinValues),
+                      dim3(kJoinThreads), 0, st, p);
 }
 
 template <typename T>
-cudaError_t launch(const AttnArgs& p, int D, bool split, cudaStream_t st) {
+cudaError_t launch(const AttnArgs& p, int D, cudaStream_t st) {
   const bool wide = p.group > 8;
-  if (D == 64) return wide ? launch_shape<T, 64, 2>(p, split, st) : launch_shape<T, 64, 1>(p, split, st);
-  if (D == 128) return wide ? launch_shape<T, 128, 2>(p, split, st) : launch_shape<T, 128, 1>(p, split, st);
-  return wide ? launch_shape<T, 256, 2>(p, split, st) : launch_shape<T, 256, 1>(p, split, st);
+  if (D == 64) return wide ? launch_shape<T, 64, 2>(p, st) : launch_shape<T, 64, 1>(p, st);
+  if (D == 128) return wide ? launch_shape<T, 128, 2>(p, st) : launch_shape<T, 128, 1>(p, st);
+  return wide ? launch_shape<T, 256, 2>(p, st) : launch_shape<T, 256, 1>(p, st);
 }
 
 }  // namespace
@@ -611,8 +633,9 @@ extern "C" {
 
 size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D, int max_tokens) {
   if (B < 1 || HQ < 1 || HKV < 1 || HQ % HKV != 0 || (D != 64 && D != 128 && D != 256)) return 0;
-  if (max_tokens <= kBlock) return 0;    // no row is ever cut
-  return static_cast<size_t>(2 * grid_of(B, HQ, HKV, D, max_tokens)) * heads_of(HQ / HKV) * (D + 2) * 4;
+  if (max_tokens <= block_of(D)) return 0;    // no row is ever cut
+  return static_cast<size_t>(grid_of(B, HQ, HKV, D, max_tokens)) *
+         (2 * static_cast<size_t>(heads_of(HQ / HKV)) * (D + 2) * 4 + sizeof(int4));
 }
 
 int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
@@ -663,11 +686,15 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   p.sinks = window > 0 ? num_sinks : 0;
   p.tiles = (p.group + heads_of(p.group) - 1) / heads_of(p.group);
   p.grid = static_cast<int>(grid_of(B, HQ, HKV, D, max_tokens));
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<size_t>(2 * p.grid) * heads_of(p.group) * D;
+  if (need > 0) {
+    p.cut = static_cast<int4*>(workspace);
+    p.part_o = reinterpret_cast<float*>(p.cut + p.grid);
+    p.part_ml = p.part_o + static_cast<size_t>(2 * p.grid) * heads_of(p.group) * D;
+  }
+  p.twin = p.k_page == p.v_page && p.k_tok == p.v_tok;
   div_constants(static_cast<uint32_t>(page_size), p.page_mul, p.page_shift);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, need > 0, st) : launch<__half>(p, D, need > 0, st);
+  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, st) : launch<__half>(p, D, st);
   return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 
