@@ -22,10 +22,10 @@ using namespace gdn_serving;
 
 constexpr int kMaxBeams = 64, kMaxSelected = 64;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kSlice = 3072;     // 16-byte vectors of logits a CTA holds: 48 KB, four CTAs per SM
-constexpr int kList = 512;       // candidates of a slice that are ranked
+constexpr int kBatch = 4;        // 16-byte vectors of logits a thread takes at a time
+constexpr int kList = 1024;      // vectors, then candidates, that a slice gathers
 constexpr int kMergeThreads = 512;
-constexpr int kHeadItems = 1024; // of the merge's bound
+constexpr int kHeadItems = 256;  // of the merge's bound
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BeamArgs {
@@ -93,26 +93,71 @@ template <typename T> struct Vec {
 
 // ------------------------------------------------------------------ one slice of a row
 //
-// A CTA copies its slice of a row to shared memory, all copies in flight at once; from there
-// it takes the maximum, then the sum of exponentials and the n best, so the logits cross HBM
-// once.  The n-th largest of the threads' maxima, T, is a lower bound of the slice's n-th
-// best; what is >= T, rarely more than a few n values, is gathered and ranked.
+// One pass over the slice.  Every thread keeps its own running maximum and its sum of
+// exponentials relative to it, so the loop has no barrier; its next batch of vectors is in
+// flight while it works on one.  The first batch is a sample spread over the slice: with
+// r = ceil(n / warps), the smallest of the warps' r-th largest lane maxima, T, has n logits
+// at or above it.  Vectors that reach T are set aside as they are; at the end the n-th
+// largest of their maxima is a sharper bound, and what reaches that is ranked.
 //
 // Bound: HBM for fp32; for 16-bit logits the exponentials come near it (12.3 logits a clock
 // and SM at the measured copy rate, of 16 exponentials), so an element costs one unpack,
-// one fused multiply-add, one exponential, one addition and 1/8 of a packed maximum,
-// compare and two 16-byte loads.
+// one fused multiply-add, one exponential, one addition and parts of packed maxima.
 
 struct SliceShared {
-  unsigned long long list[kList];
-  float lane_max[kThreads];      // each warp's lane maxima, descending
+  uint4 vec[kList];                // vectors that reach T
+  int at[kList];                   // their places in the row
+  unsigned long long list[kList];  // keys of candidates
   float red[kWarps];
   double sum[kWarps];
   int scan[kWarps];
   unsigned long long best[kWarps];
-  int count;
+  float sample[kThreads];        // of the keys, where they overflow
+  int count, keys;
   float bound;
 };
+
+// Sums of 2^(x log2 e - c) in two packed chains; one fused multiply-add and one addition do
+// two elements.
+struct ExpSum {
+  unsigned long long s[2] = {0ull, 0ull};
+  static __device__ __forceinline__ unsigned long long pack(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+  }
+  static __device__ __forceinline__ void unpack(unsigned long long x, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+  }
+  __device__ __forceinline__ void add(int chain, float x0, float x1, unsigned long long minus_c) {
+    unsigned long long t;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t) : "l"(pack(x0, x1)), "l"(pack(kLog2e, kLog2e)), "l"(minus_c));
+    float a, b;
+    unpack(t, a, b);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s[chain]) : "l"(pack(exp2_fast(a), exp2_fast(b))));
+  }
+  __device__ __forceinline__ void scale(float f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(s[i]) : "l"(pack(f, f)));
+  }
+  __device__ __forceinline__ float total() const {
+    float a, b, c, d;
+    unpack(s[0], a, b);
+    unpack(s[1], c, d);
+    return (a + b) + (c + d);
+  }
+};
+
+// Any two different logits this large are so far apart that only the largest counts.
+constexpr float kHuge = 1e30f;
+
+// One place of a list.  Few lanes of a warp ask at a time, so each asks for itself.
+__device__ __forceinline__ int next_place(int* count) {
+  int at;
+  asm volatile("atom.shared.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(smem_addr(count)) : "memory");
+  return at;
+}
 
 // Descending bitonic sort of one value per lane.
 __device__ __forceinline__ float sort_lanes(float x, int lane) {
@@ -143,95 +188,129 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs p) {
   using V = Vec<T>;
   constexpr int E = V::kN;
-  extern __shared__ __align__(16) unsigned char smem[];
-  V* held = reinterpret_cast<V*>(smem);
   __shared__ SliceShared sh;
-  const int slice = blockIdx.x % p.slices, row = blockIdx.x / p.slices, b = row / p.K, i = row % p.K;
+  const int slice = blockIdx.y, row = blockIdx.x, b = row / p.K, i = row - b * p.K;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   grid_trigger();                // the merge may take its place once the last slices run
   // a finished or dead beam's logits decide nothing
   if ((p.finished && p.finished[row]) || !isfinite(p.scores[row])) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + b * p.stride_batch + i * p.stride_beam;
   // the row as aligned 16-byte vectors; vector c holds tokens c E - mis ...; the first and the
-  // last may be partial
+  // last may be partial and are handled one by one
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int vecs = (p.V + mis + E - 1) / E;
-  const int v0 = static_cast<int>(static_cast<long long>(vecs) * slice / p.slices);
-  const int v1 = static_cast<int>(static_cast<long long>(vecs) * (slice + 1) / p.slices);
+  const int each = vecs / p.slices, more = vecs - each * p.slices;   // the first `more` get one more
+  const int v0 = slice * each + min(slice, more), v1 = v0 + each + (slice < more ? 1 : 0);
+  const int lo = v0 == 0 && mis ? 1 : v0, hi = v1 == vecs && (p.V + mis) % E ? v1 - 1 : v1;
   const uint4* base = reinterpret_cast<const uint4*>(x - mis);
-  const int nv = v1 - v0;
-  for (int c = tid; c < nv; c += kThreads) {
-    const int t0 = (v0 + c) * E - mis;
-    if (t0 >= 0 && t0 + E <= p.V) {
-      copy16_async(smem_addr(held + c), base + v0 + c, true);
-    } else {
+  // batch j of thread tid: whole vectors lo + (j + k batches) 256 + tid, k < kBatch
+  const int batches = max(1, (hi - lo + kThreads * kBatch - 1) / (kThreads * kBatch));
+  V none;
+  {
+    T inf[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        reinterpret_cast<T*>(held + c)[e] = (t0 + e >= 0 && t0 + e < p.V) ? x[t0 + e] : T(-INFINITY);
-    }
+    for (int e = 0; e < E; ++e) inf[e] = T(-INFINITY);
+    none.u = *reinterpret_cast<uint4*>(inf);
   }
-  copy_commit();
+  auto load = [&](V (&v)[kBatch], int j) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int c = lo + (j + k * batches) * kThreads + tid;
+      v[k] = none;
+      if (c < hi) v[k].u = __ldcs(base + c);
+    }
+  };
+  V v[kBatch];
+  load(v, 0);
   if (tid == 0) {
-    sh.count = 0;
+    sh.count = sh.keys = 0;
     sh.bound = -INFINITY;
   }
-  copy_wait<0>();                // a thread looks at its own vectors only: no barrier
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int c = tid; c < nv; c += kThreads) m = fmaxf(m, held[c].largest());
-  const float mine = sort_lanes(m, lane);
-  sh.lane_max[tid] = mine;
-  if (lane == 0) sh.red[warp] = mine;
+  float m = -INFINITY;           // this thread's largest logit
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) m = fmaxf(m, v[k].largest());
+  {
+    const float sorted = sort_lanes(m, lane);
+    if (lane == (p.n + kWarps - 1) / kWarps - 1) sh.red[warp] = sorted;
+  }
+  __syncthreads();
+  float bound = sh.red[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.red[w]);
+  unsigned long long* out = p.keys + (static_cast<long long>(row) * p.slices + slice) * p.n;
+  // s = sum of 2^(x log2 e - c), c = m log2 e as rounded (within +-kHuge), in four chains
+  float c0 = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
+  ExpSum sums;
+  bound = fmaxf(bound, -FLT_MAX);   // vectors of -inf alone never count
+  auto set_aside = [&](const V& w, int c) {
+    const int at = next_place(&sh.count);
+    if (at < kList) {
+      sh.vec[at] = w.u;
+      sh.at[at] = c;
+    }
+  };
+  auto raise = [&](float top) {
+    m = top;
+    const float c1 = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e, f = exp2_fast(c0 - c1);
+    sums.scale(f);
+    c0 = c1;
+  };
+  if (lo != v0 || hi != v1) {    // partial vectors: two threads of the first and last slice
+    const int c = tid == 0 && lo != v0 ? v0 : tid == 32 && hi != v1 ? v1 - 1 : -1;
+    if (c >= 0) {
+      V w = none;
+      T tmp[E];
+      *reinterpret_cast<uint4*>(tmp) = none.u;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int t = c * E - mis + e;
+        if (t >= 0 && t < p.V) tmp[e] = x[t];
+      }
+      w.u = *reinterpret_cast<uint4*>(tmp);
+      if (w.largest() > m) raise(w.largest());
+#pragma unroll
+      for (int e = 0; e < E; e += 2) sums.add(e / 2 % 2, w.get(e), w.get(e + 1), ExpSum::pack(-c0, -c0));
+      if (w.largest() >= bound) set_aside(w, c);
+    }
+  }
+  for (int j = 0;; ++j) {
+    V next[kBatch];
+    if (j + 1 < batches) load(next, j + 1);
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float t = v[k].largest();
+      if (t >= bound) set_aside(v[k], lo + (j + k * batches) * kThreads + tid);
+      top = fmaxf(top, t);
+    }
+    if (top > m) raise(top);
+    const unsigned long long minus_c = ExpSum::pack(-c0, -c0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+      for (int e = 0; e < E; e += 2) sums.add(e / 2 % 2, v[k].get(e), v[k].get(e + 1), minus_c);
+    if (j + 1 >= batches) break;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) v[k] = next[k];
+  }
+  // the CTA's maximum and sum
+  const float wm = warp_max(m);
+  if (lane == 0) sh.red[warp] = wm;
   __syncthreads();
   m = sh.red[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.red[w]);
-  unsigned long long* out = p.keys + (static_cast<long long>(row) * p.slices + slice) * p.n;
-  // rank of this thread's entry among all lane maxima: its place in its own warp's list and,
-  // by binary search, the entries before it in the others (equal ones: lower warp first)
-  if (lane < p.n) {
-    int rank = lane;
-#pragma unroll
-    for (int o = 1; o < kWarps; ++o) {
-      const int w = (warp + o) % kWarps;
-      const float* other = sh.lane_max + w * 32;
-      int lo = 0;
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) {
-        const float y = other[lo + s - 1];
-        if (w < warp ? y >= mine : y > mine) lo += s;
-      }
-      const float y = other[lo];
-      rank += lo + (w < warp ? y >= mine : y > mine);
-    }
-    if (rank == p.n - 1) sh.bound = mine;
-  }
-  __syncthreads();
-  // sum of 2^(x f - c) with f = log2 e and c = m f as rounded; what the rounding of c took is
-  // put back once at the end.  Four chains of additions per thread.  Where m f could
-  // overflow (a slice masked with the type's lowest value) two different logits are so far
-  // apart that any small f gives the same sum.
-  const float base_m = isfinite(m) ? m : 0.f, f = fabsf(base_m) < 1e30f ? kLog2e : 0x1p-64f;
-  const float c0 = base_m * f;
-  const float bound = sh.bound;
-  float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int c = tid; c < nv; c += kThreads) {
-    const V v = held[c];
-#pragma unroll
-    for (int e = 0; e < E; ++e) s4[e % 4] += exp2_fast(fmaf(v.get(e), f, -c0));
-    if (v.largest() >= bound) {
-      const int t0 = (v0 + c) * E - mis;
-      for (int e = 0; e < E; ++e) {
-        const float y = to_f(reinterpret_cast<const T*>(held + c)[e]);
-        if (y >= bound && y > -INFINITY) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kList) sh.list[at] = make_key(y, t0 + e);
-        }
-      }
+  const float held = fminf(fmaxf(m, -kHuge), kHuge), c1 = held * kLog2e;
+  double s = static_cast<double>(sums.total()) *
+             static_cast<double>(exp2_fast(c0 - c1));
+  const int e0 = max(0, v0 * E - mis), e1 = min(p.V, v1 * E - mis);   // the slice's tokens
+  if (held != m && isfinite(m)) {
+    s = 0.0;
+    for (int t = e0 + tid; t < e1; t += kThreads) {
+      const float y = to_f(x[t]);
+      s += isnan(y) ? NAN : y == m ? 1.0 : 0.0;
     }
   }
-  double s = static_cast<double>(s4[0] + s4[1]) + static_cast<double>(s4[2] + s4[3]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sh.sum[warp] = s;
@@ -240,28 +319,80 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     s = sh.sum[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) s += sh.sum[w];
-    s *= static_cast<double>(exp2f(-fmaf(base_m, f, -c0)));
+    if (held == m) s *= static_cast<double>(exp2f(-fmaf(held, kLog2e, -c1)));   // what c's rounding took
     p.sums[static_cast<long long>(row) * p.slices + slice] = make_float2(m, static_cast<float>(s));
   }
-  if (sh.count <= kList) {
-    write_ranked(sh.list, sh.count, p.n, out);
+  // a sharper bound from up to 256 of the vectors set aside, as before: whole warps of them
+  const int aside = min(sh.count, kList), wide = min(aside, kThreads) / 32;
+  const int nth = wide > 0 ? (p.n + wide - 1) / wide : 33;
+  if (warp < wide && nth <= 32) {
+    const float sorted = sort_lanes(V{sh.vec[tid]}.largest(), lane);
+    if (lane == nth - 1) sh.red[warp] = sorted;
+  }
+  __syncthreads();
+  if (nth <= 32) {               // at least the bound before
+    bound = sh.red[0];
+    for (int w = 1; w < wide; ++w) bound = fminf(bound, sh.red[w]);
+  }
+  bool full = sh.count > kList;
+  if (!full) {
+    for (int f = tid; f < aside * E; f += kThreads) {
+      const float y = to_f(reinterpret_cast<const T*>(sh.vec)[f]);
+      if (y >= bound) {
+        const int at = next_place(&sh.keys);
+        if (at < kList) sh.list[at] = make_key(y, sh.at[f / E] * E - mis + f % E);
+      }
+    }
+    __syncthreads();
+    full = sh.keys > kList;
+  }
+  // The sample missed where the large ones are: read the slice again with the higher bound,
+  // raised from what was gathered until it fits or does not rise.
+  if (full) {
+    float last = -INFINITY;      // below any bound
+    while (bound > last) {
+      __syncthreads();
+      if (tid == 0) sh.keys = 0;
+      __syncthreads();
+      for (int t = e0 + tid; t < e1; t += kThreads) {
+        const float z = to_f(x[t]);
+        if (z >= bound) {
+          const int at = atomicAdd(&sh.keys, 1);
+          if (at < kList) sh.list[at] = make_key(z, t);
+        }
+      }
+      __syncthreads();
+      full = sh.keys > kList;
+      if (!full) break;
+      const float y = key_logit(sh.list[tid]);
+      sh.sample[tid] = y;
+      __syncthreads();
+      int rank = 0;
+      for (int o = 0; o < kThreads; ++o) rank += sh.sample[o] > y || (sh.sample[o] == y && o < tid);
+      if (rank == p.n - 1) sh.bound = y;
+      __syncthreads();
+      last = bound;
+      bound = sh.bound;
+    }
+  }
+  if (!full) {
+    write_ranked(sh.list, sh.keys, p.n, out);
     return;
   }
   // Rare: many values equal to the bound (a mask of the type's lowest value, coarse logits).
   // Those above it, then the first n equal ones in order of tokens, read again from memory.
-  const int e0 = max(0, v0 * E - mis), e1 = min(p.V, v1 * E - mis);
   __syncthreads();
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.keys = 0;
   __syncthreads();
   for (int t = e0 + tid; t < e1; t += kThreads) {
     const float y = to_f(x[t]);
     if (y > bound) {
-      const int at = atomicAdd(&sh.count, 1);
+      const int at = atomicAdd(&sh.keys, 1);
       if (at < kList) sh.list[at] = make_key(y, t);
     }
   }
   __syncthreads();
-  const int above = sh.count;
+  const int above = sh.keys;
   if (above + p.n <= kList) {
     int have = 0;
     for (int t1 = e0; t1 < e1 && have < p.n; t1 += kThreads) {
@@ -311,128 +442,188 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 // ------------------------------------------------------------------ the merge
 //
 // One CTA per request.  The n-th best of the slices' first candidates is a lower bound of the
-// result's n-th best.  What reaches it gets its rank, among its beam's slices and then among
-// all beams, by binary searches in the sorted lists; whoever has a rank below n writes
-// itself to that place, so nothing depends on the order in which threads run.
+// result's n-th best.  What reaches it is gathered, and whoever has fewer than n better ones
+// writes itself to that place, so nothing depends on the order in which threads run.  With
+// more of them than the list holds (many equal scores) the ranks come from binary searches
+// in the sorted lists instead.
 
-__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArgs p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  double* score = reinterpret_cast<double*>(smem);                   // [K, n] descending
-  int* token = reinterpret_cast<int*>(score + p.K * p.n);            // [K, n]
-  double* lse = reinterpret_cast<double*>(token + p.K * p.n + (p.K * p.n & 1));   // [K]
-  __shared__ int alive;
-  __shared__ double head[kHeadItems], bound;
+constexpr int kMergeList = 1024;
+
+struct MergeItem {
+  unsigned long long score;      // of the 64-bit score, in an order-preserving form
+  unsigned long long key;        // of its logit and token; ~0 for a finished beam's one
+  int beam;
+};
+
+__device__ __forceinline__ unsigned long long ordered(double x) {
+  const unsigned long long u = __double_as_longlong(x + 0.0);   // -0 and +0 are equal
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double from_ordered(unsigned long long o) {
+  return __longlong_as_double(o >> 63 ? o & 0x7fffffffffffffffull : ~o);
+}
+
+// ln(t) for t >= 1: the fraction's logarithm in fp32 (6e-8), the exponent's in 64 bits
+__device__ __forceinline__ double ln_sum(double t) {
+  const unsigned long long u = __double_as_longlong(t);
+  const int e = static_cast<int>(u >> 52) - 1023;
+  const double f = __longlong_as_double((u & 0x000fffffffffffffull) | 0x3ff0000000000000ull);
+  return e * 0.69314718055994530942 + static_cast<double>(logf(static_cast<float>(f)));
+}
+
+// sum over a group of 8 lanes; groups of one warp may have left the loop
+__device__ __forceinline__ int sum8(int x) {
+  const uint32_t mask = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
+  return x;
+}
+
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
+  __shared__ double lse[kMaxBeams], cum[kMaxBeams], bound;
+  __shared__ unsigned long long head[kHeadItems];
+  __shared__ MergeItem item[kMergeList];
+  __shared__ int count, alive;
+  __shared__ bool done[kMaxBeams];
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int per_beam = p.slices * p.n;
-  for (int f = tid; f < p.K * p.n; f += kMergeThreads) score[f] = -INFINITY;
+  const int per_beam = p.slices * p.n, lists = p.K * p.slices, total = lists * p.n;
   if (tid == 0) {
-    alive = 0;
+    count = alive = 0;
     bound = -INFINITY;
   }
+  if (tid < p.K) {
+    const float c = p.scores[b * p.K + tid];
+    cum[tid] = c;
+    done[tid] = p.finished && p.finished[b * p.K + tid];
+  }
+  __syncthreads();
   grid_wait();
   for (int i = warp; i < p.K; i += kMergeThreads / 32) {
-    const int row = b * p.K + i;
-    const bool skip = (p.finished && p.finished[row]) || !isfinite(p.scores[row]);
-    double l = NAN;
-    if (!skip) {
-      const float2* sums = p.sums + static_cast<long long>(row) * p.slices;
+    double l = NAN;                     // not finite: a beam without candidates of its own
+    if (!done[i] && isfinite(cum[i])) {
+      const float2* sums = p.sums + (static_cast<long long>(b) * p.K + i) * p.slices;
       float m = -INFINITY;
       for (int s = lane; s < p.slices; s += 32) m = fmaxf(m, sums[s].x);
       m = warp_max(m);
       double t = 0.0;
       for (int s = lane; s < p.slices; s += 32) {
         const float2 ms = sums[s];
-        if (ms.x > -INFINITY || isnan(ms.y)) t += ms.y * exp(static_cast<double>(ms.x) - m);
+        if (ms.x > -INFINITY || isnan(ms.y))
+          t += static_cast<double>(ms.y) * static_cast<double>(exp2f((ms.x - m) * kLog2e));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      l = m + log(t);
+      if (isfinite(m) && t >= 0.5 && t < 1e300) l = m + ln_sum(t);
     }
-    if (lane == 0) lse[i] = l;          // not finite: a row that holds no candidate
+    if (lane == 0) lse[i] = l;
   }
   __syncthreads();
+  const unsigned long long* all = p.keys + static_cast<long long>(b) * total;
+  auto score_of = [&](int i, unsigned long long k) {
+    return cum[i] + (static_cast<double>(key_logit(k)) - lse[i]);
+  };
   // the first `depth` candidates of every slice (of as many slices as fit), at least n where
   // there are as many
-  const unsigned long long* all = p.keys + static_cast<long long>(b) * p.K * per_beam;
-  const int lists = p.K * p.slices, depth = (p.n + lists - 1) / lists;
-  const int items = min(lists * depth, kHeadItems);
-  for (int f = tid; f < items; f += kMergeThreads) {
-    const int list = f % lists, i = list / p.slices, r = f / lists;
-    double sc = -INFINITY;
-    if (isfinite(lse[i])) {
-      const unsigned long long k = all[list * p.n + r];
-      if (k) sc = static_cast<double>(p.scores[b * p.K + i]) + (static_cast<double>(key_logit(k)) - lse[i]);
-    }
-    head[f] = sc;
+  const int depth = (p.n + lists - 1) / lists, items = min(lists * depth, kHeadItems);
+  if (tid < items) {
+    const int list = tid % lists, i = list / p.slices;
+    const unsigned long long k = isfinite(lse[i]) ? all[list * p.n + tid / lists] : 0;
+    head[tid] = ordered(k ? score_of(i, k) : -INFINITY);
   }
   __syncthreads();
-  for (int f = tid; f < items; f += kMergeThreads) {
-    const double sc = head[f];
+  // eight threads count for one
+  for (int f = tid / 8; f < items; f += kMergeThreads / 8) {
+    const unsigned long long sc = head[f];
     int rank = 0;
-    for (int o = 0; o < items; ++o) rank += head[o] > sc || (head[o] == sc && o < f);
-    if (rank == p.n - 1) bound = sc;
+    for (int o = tid % 8; o < items; o += 8) rank += (head[o] > sc) | ((head[o] == sc) & (o < f));
+    rank = sum8(rank);
+    if (rank == p.n - 1) bound = from_ordered(sc);
   }
   __syncthreads();
-  // each beam's candidates at or above the bound, in order
-  for (int f = tid; f < p.K * per_beam; f += kMergeThreads) {
-    const int i = f / per_beam, at = f % per_beam, s = at / p.n, r = at % p.n;
-    if (!isfinite(lse[i])) continue;
-    const unsigned long long* keys = all + i * per_beam;
-    const unsigned long long k = keys[at];
-    if (k == 0) continue;
-    const double sc =
-        static_cast<double>(p.scores[b * p.K + i]) + (static_cast<double>(key_logit(k)) - lse[i]);
-    if (!(sc >= bound)) continue;
-    int rank = r;
-    for (int o = 0; o < p.slices && rank < p.n; ++o) {
-      if (o == s) continue;
-      int lo = 0, hi = p.n;              // keys of a beam are all different
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (keys[o * p.n + mid] > k) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank < p.n) {
-      score[i * p.n + rank] = sc;
-      token[i * p.n + rank] = key_token(k);
-    }
-  }
-  for (int i = tid; i < p.K; i += kMergeThreads)
-    if (p.finished && p.finished[b * p.K + i] && isfinite(p.scores[b * p.K + i])) {
-      score[i * p.n] = p.scores[b * p.K + i];
-      token[i * p.n] = p.eos;
-    }
-  __syncthreads();
-  // the n best of all beams
+  const double low = bound;
   int valid = 0;
-  for (int f = tid; f < p.K * p.n; f += kMergeThreads) {
-    const int i = f / p.n;
-    const double sc = score[f];
-    if (!(sc > -INFINITY)) continue;
-    ++valid;
-    int rank = f % p.n;
-    for (int o = 0; o < p.K && rank < p.n; ++o) {
-      if (o == i) continue;
-      int lo = 0, hi = p.n;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        const double y = score[o * p.n + mid];
-        if (o < i ? y >= sc : y > sc) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
+  for (int f0 = 0; f0 < total; f0 += 4 * kMergeThreads) {
+    unsigned long long k[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int f = f0 + u * kMergeThreads + tid;
+      k[u] = f < total && isfinite(lse[f / per_beam]) ? all[f] : 0;
     }
-    if (rank < p.n) {
-      const long long at = static_cast<long long>(b) * p.n + rank;
-      p.tokens[at] = token[f];
-      p.parents[at] = i;
-      p.out_scores[at] = static_cast<float>(sc);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = (f0 + u * kMergeThreads + tid) / per_beam;
+      if (k[u] == 0) continue;
+      ++valid;
+      const double sc = score_of(i, k[u]);
+      if (!(sc >= low)) continue;
+      const int at = atomicAdd(&count, 1);
+      if (at < kMergeList) item[at] = MergeItem{ordered(sc), k[u], i};
+    }
+  }
+  if (tid < p.K && done[tid] && isfinite(cum[tid])) {
+    ++valid;
+    if (cum[tid] >= low) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kMergeList) item[at] = MergeItem{ordered(cum[tid]), ~0ull, tid};
     }
   }
   if (valid) atomicAdd(&alive, valid);
   __syncthreads();
+  auto place = [&](int rank, double sc, int i, unsigned long long k) {
+    const long long at = static_cast<long long>(b) * p.n + rank;
+    p.tokens[at] = k == ~0ull ? p.eos : key_token(k);
+    p.parents[at] = i;
+    p.out_scores[at] = static_cast<float>(sc);
+  };
+  if (count <= kMergeList) {
+    for (int f = tid / 8; f < count; f += kMergeThreads / 8) {
+      const MergeItem me = item[f];
+      int rank = 0;
+      for (int o = tid % 8; o < count; o += 8) {
+        const MergeItem it = item[o];
+        rank += (it.score > me.score) |
+                ((it.score == me.score) & ((it.beam < me.beam) | ((it.beam == me.beam) & (it.key > me.key))));
+      }
+      rank = sum8(rank);
+      if (rank < p.n && tid % 8 == 0) place(rank, from_ordered(me.score), me.beam, me.key);
+    }
+  } else {
+    // better ones in every list: higher scores, and equal ones of lower beams or, within the
+    // beam, larger keys
+    for (int f = tid; f < total + p.K; f += kMergeThreads) {
+      const int i = f < total ? f / per_beam : f - total;
+      unsigned long long k = ~0ull;
+      double sc = cum[i];
+      if (f < total) {
+        k = isfinite(lse[i]) ? all[f] : 0;
+        if (k == 0) continue;
+        sc = score_of(i, k);
+      } else if (!done[i]) {
+        continue;
+      }
+      if (!(sc >= low) || !isfinite(sc)) continue;
+      int rank = 0;
+      for (int o = 0; o < p.K && rank < p.n; ++o) {
+        if (done[o]) {
+          rank += isfinite(cum[o]) && (cum[o] > sc || (cum[o] == sc && o < i));
+          continue;
+        }
+        if (!isfinite(lse[o])) continue;
+        for (int l = o * p.slices; l < (o + 1) * p.slices && rank < p.n; ++l) {
+          int lo = 0, hi = p.n;
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            const unsigned long long q = all[l * p.n + mid];
+            const double y = q ? score_of(o, q) : -INFINITY;
+            if (y > sc || (y == sc && (o < i || (o == i && q > k)))) lo = mid + 1;
+            else hi = mid;
+          }
+          rank += lo;
+        }
+      }
+      if (rank < p.n) place(rank, sc, i, k);
+    }
+  }
   for (int r = alive + tid; r < p.n; r += kMergeThreads) {
     const long long at = static_cast<long long>(b) * p.n + r;
     p.tokens[at] = -1;
@@ -443,31 +634,21 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamArg
 
 // ------------------------------------------------------------------ host
 
-// Slices of a row of 16-byte vectors with `per` logits: as few as a CTA holds, more while
-// the rows alone do not give every SM two CTAs and a slice keeps a vector for each thread.
+// Slices of a row of 16-byte vectors with `per` logits: more while the rows alone do not
+// give every SM two CTAs and a slice keeps a vector for each thread.
 int slices_of(long long rows, int V, int per) {
   const int vecs = V / per + 2;              // of an unaligned row
-  int s = (vecs + kSlice - 1) / kSlice;
+  int s = 1;
   while (rows * s < 2 * kSMs && vecs / (2 * s) >= kThreads) s *= 2;
+    while (rows * s < 12 * kSMs && vecs / (s + 1) >= 4 * kThreads * kBatch) ++s;
   return s;
 }
 
 template <typename T>
 int launch(const BeamArgs& p, cudaStream_t st) {
-  const int vecs = p.V / Vec<T>::kN + 2;
-  const size_t held = static_cast<size_t>(vecs / p.slices + 1) * 16;   // of the largest slice
-  if (held > 40 * 1024 &&
-      cudaFuncSetAttribute(beam_slice_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (kSlice + 1) * 16) != cudaSuccess)
-    return GDN_ERR_LAUNCH;
-  beam_slice_kernel<T><<<p.slices * p.B * p.K, kThreads, held, st>>>(p);
+  beam_slice_kernel<T><<<dim3(p.B * p.K, p.slices), kThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
-  const size_t smem = static_cast<size_t>(p.K) * (p.n * 12 + 8) + 8;
-  if (smem > 32 * 1024 &&
-      cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem)) != cudaSuccess)
-    return GDN_ERR_LAUNCH;
-  return launch_after(beam_merge_kernel, dim3(p.B), dim3(kMergeThreads), smem, st, p) == cudaSuccess
+  return launch_after(beam_merge_kernel, dim3(p.B), dim3(kMergeThreads), 0, st, p) == cudaSuccess
              ? GDN_OK : GDN_ERR_LAUNCH;
 }
 
@@ -496,9 +677,7 @@ int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch, int64_t
   if (!aligned(logits, dtype == GDN_DTYPE_FP32 ? 4 : 2) || !aligned(scores, 4) || !aligned(tokens, 4) ||
       !aligned(parents, 4) || !aligned(new_scores, 4) || !aligned(workspace, 16))
     return GDN_ERR_ALIGN;
-  if (static_cast<long long>(B) * K * std::max(slices_of(1LL * B * K, V, 4), slices_of(1LL * B * K, V, 8)) >
-      0x7fffffffLL)
-    return GDN_ERR_SHAPE;
+  if (V > (1 << 26)) return GDN_ERR_SHAPE;           // keeps the slices of a row below 2^16
   if (workspace_bytes < gdn_beam_select_workspace_bytes(B, K, V, n)) return GDN_ERR_SHAPE;
   BeamArgs p{};
   p.logits = logits; p.scores = scores; p.finished = finished; p.tokens = tokens;
