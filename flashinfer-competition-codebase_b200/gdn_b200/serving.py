@@ -18,44 +18,80 @@ different streams, and graphs captured from them, never share one.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .ops import _BF16, _F32, _check, _index_tensor, _ptr, _stream_handle
+from .ops import _BF16, _F32, _check, _index_tensor, _ptr
 
 _I32 = torch.int32
+_BOOL = torch.bool
 _DTYPE_CODES = {_BF16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, _F32: _lib.DTYPE_FP32}
 
 Pools = Union[torch.Tensor, Sequence[torch.Tensor]]
 
 
+# The small calls are bound by host work (a launch takes about 3 us), so the common case of
+# each check is one chain of comparisons, and the stream and device come from torch's
+# cheapest accessors (72 ns against 2.2 us for torch.cuda.current_stream).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """One library call on the device's current stream (the last argument)."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _raw_stream(index))
+
+
+def _need(t, name: str, dtype: torch.dtype, shape, device) -> None:
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.device == device
+            and (shape is None or t.shape == shape) and t.is_contiguous()):
+        return
+    _check(t, name, dtype, shape, device)
+
+
 def _check_counter(bad_index_count, device) -> None:
     if bad_index_count is not None:
-        _check(bad_index_count, "bad_index_count", _I32, (1,), device)
+        _need(bad_index_count, "bad_index_count", _I32, (1,), device)
 
 
-def _check_cache(cache: torch.Tensor, name: str, dtype, HKV: int, D: int, device) -> list:
+@lru_cache(maxsize=256)
+def _int64s(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(name: str, *sizes) -> int:
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
+def _check_cache(cache: torch.Tensor, name: str, dtype, HKV: int, D: int, device):
     if not isinstance(cache, torch.Tensor) or cache.dim() != 4:
         raise ValueError(f"{name} must be 4-D [num_pages, page_size, num_kv_heads, head_dim]")
     if cache.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {cache.dtype}")
     if not cache.is_cuda or cache.device != device:
         raise ValueError(f"{name} is on {cache.device}, expected {device}")
-    if tuple(cache.shape[2:]) != (HKV, D):
-        raise ValueError(f"{name} must end in ({HKV}, {D}), got {tuple(cache.shape)}")
-    if cache.stride(3) != 1:
+    shape, strides = cache.shape, cache.stride()
+    if shape[2] != HKV or shape[3] != D:
+        raise ValueError(f"{name} must end in ({HKV}, {D}), got {tuple(shape)}")
+    if strides[3] != 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
-    strides = [cache.stride(i) if cache.shape[i] > 1 else 0 for i in range(3)]
-    if any(s <= 0 and n > 1 for s, n in zip(strides, cache.shape)):
+    strides = tuple(s if n > 1 else 0 for s, n in zip(strides[:3], shape))
+    if any(s <= 0 and n > 1 for s, n in zip(strides, shape)):
         raise ValueError(f"{name} must not be expanded (a stride of 0)")
-    if any(s % 8 for s in strides) or cache.data_ptr() % 16:
+    if (strides[0] | strides[1] | strides[2]) % 8 or cache.data_ptr() % 16:
         raise ValueError(f"{name} needs 16-byte aligned rows (strides a multiple of 8 elements)")
     return strides
 
 
-@torch.no_grad()
 def paged_attention_decode(
     q, k_cache, v_cache, block_tables, seq_lens, k=None, v=None, scale=None, window: int = 0,
     num_sinks: int = 0, output=None, bad_index_count=None,
@@ -85,7 +121,7 @@ def paged_attention_decode(
         raise TypeError(f"q must be bfloat16 or float16, got {dt}")
     if D not in (64, 128, 256):
         raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
-    _check(q, "q", dt, None, dev)
+    _need(q, "q", dt, None, dev)
     HKV = k_cache.shape[2] if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 0
     if HKV < 1 or HQ < 1 or HQ % HKV != 0:
         raise ValueError(f"num heads ({HQ}) must be a multiple of num kv heads ({HKV})")
@@ -109,34 +145,33 @@ def paged_attention_decode(
         raise ValueError("block_tables must have contiguous rows")
     if width * page_size > 2**31 - 2048:
         raise ValueError("block_tables hold more than 2**31 - 2048 tokens a row")
-    _check(seq_lens, "seq_lens", _I32, (B,), dev)
+    _need(seq_lens, "seq_lens", _I32, (B,), dev)
     if (k is None) != (v is None):
         raise ValueError("k and v must be provided together")
     if k is not None:
-        _check(k, "k", dt, (B, 1, HKV, D), dev)
-        _check(v, "v", dt, (B, 1, HKV, D), dev)
+        _need(k, "k", dt, (B, 1, HKV, D), dev)
+        _need(v, "v", dt, (B, 1, HKV, D), dev)
     if window < 0 or num_sinks < 0 or max(window, num_sinks) > 2**30 - 1:
         raise ValueError("window and num_sinks must be between 0 and 2**30 - 1")
     if output is None:
         output = torch.empty_like(q)
-    _check(output, "output", dt, (B, 1, HQ, D), dev)
+    else:
+        _need(output, "output", dt, (B, 1, HQ, D), dev)
     _check_counter(bad_index_count, dev)
-    lse = torch.empty((B, HQ), dtype=_F32, device=dev)
-    nbytes = int(_lib.load().gdn_paged_attention_workspace_bytes(B, HQ, HKV, D, width * page_size))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    strides = ctypes.c_int64 * 3
-    with torch.cuda.device(dev):
-        _lib.call(
-            "gdn_paged_attention_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            block_tables.data_ptr(), seq_lens.data_ptr(), _ptr(k), _ptr(v),
-            0.0 if scale is None else float(scale), int(window), int(num_sinks),
-            output.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes, _DTYPE_CODES[dt], B, HQ, HKV, D,
-            num_pages, page_size, width, block_tables.stride(0) if B > 1 else width,
-            strides(*ks), strides(*vs), _ptr(bad_index_count), _stream_handle(dev))
+    lse = q.new_empty((B, HQ), dtype=_F32)
+    nbytes = _workspace_bytes("gdn_paged_attention_workspace_bytes", B, HQ, HKV, D,
+                              width * page_size)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(
+        dev, "gdn_paged_attention_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        block_tables.data_ptr(), seq_lens.data_ptr(), _ptr(k), _ptr(v),
+        0.0 if scale is None else float(scale), int(window), int(num_sinks), output.data_ptr(),
+        lse.data_ptr(), _ptr(ws), nbytes, _DTYPE_CODES[dt], B, HQ, HKV, D, num_pages, page_size,
+        width, block_tables.stride(0) if B > 1 else width, _int64s(*ks), _int64s(*vs),
+        _ptr(bad_index_count))
     return output, lse
 
 
-@torch.no_grad()
 def beam_select(
     logits, scores, num_selected: Optional[int] = None, finished=None, eos_token: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -167,22 +202,20 @@ def beam_select(
     n = K if num_selected is None else int(num_selected)
     if n < 1 or n > 64 or K > 64:
         raise ValueError(f"beam_select takes up to 64 beams and 1 to 64 selected, got {K} and {n}")
-    _check(scores, "scores", _F32, (B, K), dev)
+    _need(scores, "scores", _F32, (B, K), dev)
     if finished is not None:
-        _check(finished, "finished", torch.bool, (B, K), dev)
+        _need(finished, "finished", _BOOL, (B, K), dev)
         if not 0 <= eos_token < V:
             raise ValueError(f"eos_token must be a token of the vocabulary, got {eos_token}")
-    tokens = torch.empty((B, n), dtype=_I32, device=dev)
-    parents = torch.empty((B, n), dtype=_I32, device=dev)
-    new_scores = torch.empty((B, n), dtype=_F32, device=dev)
-    nbytes = int(_lib.load().gdn_beam_select_workspace_bytes(B, K, V, n))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        _lib.call(
-            "gdn_beam_select", logits.data_ptr(), _DTYPE_CODES[logits.dtype], logits.stride(0),
-            logits.stride(1), scores.data_ptr(), _ptr(finished), int(eos_token), B, K, V, n,
-            tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), _ptr(ws), nbytes,
-            _stream_handle(dev))
+    new_scores = scores.new_empty((B, n))
+    tokens = torch.empty_like(new_scores, dtype=_I32)
+    parents = torch.empty_like(tokens)
+    nbytes = _workspace_bytes("gdn_beam_select_workspace_bytes", B, K, V, n)
+    ws = scores.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    stride_batch, stride_beam, _ = logits.stride()
+    _call(dev, "gdn_beam_select", logits.data_ptr(), _DTYPE_CODES[logits.dtype], stride_batch,
+          stride_beam, scores.data_ptr(), _ptr(finished), int(eos_token), B, K, V, n,
+          tokens.data_ptr(), parents.data_ptr(), new_scores.data_ptr(), _ptr(ws), nbytes)
     return tokens, parents, new_scores
 
 
@@ -191,38 +224,43 @@ class _PoolArrays:
 
     def __init__(self, pools: Pools, device=None, num_pages: Optional[int] = None):
         pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
-        if len(pools) > 32:
-            raise ValueError(f"at most 32 pools go through one call, got {len(pools)}")
+        n = len(pools)
+        if n > 32:
+            raise ValueError(f"at most 32 pools go through one call, got {n}")
+        nbytes, pitch = [], []
         for i, t in enumerate(pools):
             if not isinstance(t, torch.Tensor) or t.dim() < 2:
                 raise ValueError(f"pool {i} must be a tensor [num_pages, ...]")
             if not t.is_cuda:
                 raise ValueError(f"pool {i} must be a CUDA tensor (the B200 path has no CPU fallback)")
-            device = t.device if device is None else device
+            if device is None:
+                device = t.device
             if t.device != device:
                 raise ValueError(f"pool {i} is on {t.device}, expected {device}")
-            num_pages = t.shape[0] if num_pages is None else num_pages
-            if t.shape[0] != num_pages or num_pages < 1 or t[0].numel() < 1:
+            pages, numel = t.shape[0], t.numel()
+            if num_pages is None:
+                num_pages = pages
+            if pages != num_pages or numel < 1:
                 raise ValueError(f"pool {i} must have {num_pages} pages, got {tuple(t.shape)}")
-            if not t[0].is_contiguous():
+            if not t.is_contiguous() and not t[0].is_contiguous():
                 raise ValueError(f"pool {i} must be contiguous within a page")
-        self.device, self.num_pages, self.count = device, num_pages, len(pools)
-        nbytes = [t[0].numel() * t.element_size() for t in pools]
-        pitch = [t.stride(0) * t.element_size() if t.shape[0] > 1 else b
-                 for t, b in zip(pools, nbytes)]
-        self.ptrs = (ctypes.c_void_p * max(1, len(pools)))(*[t.data_ptr() for t in pools])
-        self.bytes = (ctypes.c_int64 * max(1, len(pools)))(*nbytes)
-        self.pitch = (ctypes.c_int64 * max(1, len(pools)))(*pitch)
+            size = t.element_size()
+            nbytes.append(numel // pages * size)
+            pitch.append(t.stride(0) * size if pages > 1 else nbytes[i])
+        self.device, self.num_pages, self.count = device, num_pages, n
+        self.ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in pools]) if n else None
+        self.bytes = _int64s(*nbytes) if n else None
+        self.pitch = _int64s(*pitch) if n else None
 
 
 def _check_refcounts(refcounts) -> Tuple[int, torch.device]:
     if not isinstance(refcounts, torch.Tensor) or refcounts.dim() != 1 or refcounts.numel() < 1:
         raise ValueError("refcounts must be a 1-D tensor [num_pages]")
-    _check(refcounts, "refcounts", _I32)
-    return refcounts.shape[0], refcounts.device
+    dev = refcounts.device
+    _need(refcounts, "refcounts", _I32, None, dev)
+    return refcounts.shape[0], dev
 
 
-@torch.no_grad()
 def copy_pages(pools: Pools, src, dst, bad_index_count=None) -> None:
     """``pool[dst[i]] = pool[src[i]]`` for all i at once, in every pool, in place.
 
@@ -243,13 +281,10 @@ def copy_pages(pools: Pools, src, dst, bad_index_count=None) -> None:
     if n > 4096:
         raise ValueError(f"at most 4096 pages are copied by one call, got {n}")
     _check_counter(bad_index_count, p.device)
-    with torch.cuda.device(p.device):
-        _lib.call("gdn_copy_pages", p.ptrs, p.bytes, p.pitch, p.count, p.num_pages,
-                  src.data_ptr(), dst.data_ptr(), n, _ptr(bad_index_count),
-                  _stream_handle(p.device))
+    _call(p.device, "gdn_copy_pages", p.ptrs, p.bytes, p.pitch, p.count, p.num_pages,
+          src.data_ptr(), dst.data_ptr(), n, _ptr(bad_index_count))
 
 
-@torch.no_grad()
 def alloc_pages(refcounts, need) -> torch.Tensor:
     """A free page for each marked entry of ``need`` [n] bool: returns pages [n] int32, the
     lowest free pages of ``refcounts`` [num_pages] int32 in order (their count becomes 1);
@@ -258,31 +293,27 @@ def alloc_pages(refcounts, need) -> torch.Tensor:
     P, dev = _check_refcounts(refcounts)
     if not isinstance(need, torch.Tensor) or need.dim() != 1:
         raise ValueError("need must be a 1-D bool tensor")
-    _check(need, "need", torch.bool, None, dev)
+    _need(need, "need", _BOOL, None, dev)
     n = need.shape[0]
-    pages = torch.empty(n, dtype=_I32, device=dev)
-    ws = torch.empty(n, dtype=_I32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("gdn_alloc_pages", refcounts.data_ptr(), P, need.data_ptr(), n,
-                  pages.data_ptr(), ws.data_ptr(), 4 * n, _stream_handle(dev))
+    pages = refcounts.new_empty(n)
+    ws = torch.empty_like(pages)
+    _call(dev, "gdn_alloc_pages", refcounts.data_ptr(), P, need.data_ptr(), n, pages.data_ptr(),
+          ws.data_ptr(), 4 * n)
     return pages
 
 
-@torch.no_grad()
 def free_pages(refcounts, pages, bad_index_count=None) -> None:
     """One reference less in ``refcounts`` for every entry of ``pages`` (int32, any shape,
     contiguous: block-table rows go in as they are, negative entries are skipped).  Entries
     >= num_pages and entries of pages without a reference left are counted in
     ``bad_index_count`` and change nothing.  C entry: ``gdn_free_pages``."""
     P, dev = _check_refcounts(refcounts)
-    _check(pages, "pages", _I32, None, dev)
+    _need(pages, "pages", _I32, None, dev)
     _check_counter(bad_index_count, dev)
-    with torch.cuda.device(dev):
-        _lib.call("gdn_free_pages", refcounts.data_ptr(), P, pages.data_ptr(), pages.numel(),
-                  _ptr(bad_index_count), _stream_handle(dev))
+    _call(dev, "gdn_free_pages", refcounts.data_ptr(), P, pages.data_ptr(), pages.numel(),
+          _ptr(bad_index_count))
 
 
-@torch.no_grad()
 def fork_pages(block_tables, seq_lens, parents, refcounts, page_size: int, pools: Pools = (),
                bad_index_count=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Forks (and thereby reorders, multiplies and drops) the sequences of a paged cache.
@@ -300,27 +331,25 @@ def fork_pages(block_tables, seq_lens, parents, refcounts, page_size: int, pools
     if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
         raise ValueError("block_tables must be 2-D [rows, width]")
     rows, width = block_tables.shape
-    _check(block_tables, "block_tables", _I32, None, dev)
-    _check(seq_lens, "seq_lens", _I32, (rows,), dev)
+    _need(block_tables, "block_tables", _I32, None, dev)
+    _need(seq_lens, "seq_lens", _I32, (rows,), dev)
     n = parents.shape[0] if isinstance(parents, torch.Tensor) and parents.dim() == 1 else 0
     parents = _index_tensor(parents, "parents", n, dev, rows)
     if page_size < 1 or width * page_size > 2**31 - 1:
         raise ValueError(f"page_size must be positive and a row below 2**31 tokens, got {page_size}")
     _check_counter(bad_index_count, dev)
     p = _PoolArrays(pools, dev, P)
-    new_tables = torch.empty((n, width), dtype=_I32, device=dev)
-    new_lens = torch.empty(n, dtype=_I32, device=dev)
-    ws = torch.empty(3 * n, dtype=_I32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call(
-            "gdn_fork_pages", block_tables.data_ptr(), width, seq_lens.data_ptr(),
-            parents.data_ptr(), refcounts.data_ptr(), new_tables.data_ptr(), new_lens.data_ptr(),
-            rows, n, width, P, int(page_size), p.ptrs, p.bytes, p.pitch, p.count, ws.data_ptr(),
-            12 * n, _ptr(bad_index_count), _stream_handle(dev))
+    new_tables = refcounts.new_empty((n, width))
+    new_lens = refcounts.new_empty(n)
+    ws = refcounts.new_empty(3 * n)
+    _call(
+        dev, "gdn_fork_pages", block_tables.data_ptr(), width, seq_lens.data_ptr(),
+        parents.data_ptr(), refcounts.data_ptr(), new_tables.data_ptr(), new_lens.data_ptr(),
+        rows, n, width, P, int(page_size), p.ptrs, p.bytes, p.pitch, p.count, ws.data_ptr(),
+        12 * n, _ptr(bad_index_count))
     return new_tables, new_lens
 
 
-@torch.no_grad()
 def compact_pages(refcounts, block_tables=None, pools: Pools = ()) -> Tuple[torch.Tensor, torch.Tensor]:
     """Closes the holes of a pool: afterwards the live pages are the first ``num_live``.
 
@@ -332,16 +361,14 @@ def compact_pages(refcounts, block_tables=None, pools: Pools = ()) -> Tuple[torc
     P, dev = _check_refcounts(refcounts)
     entries = 0
     if block_tables is not None:
-        _check(block_tables, "block_tables", _I32, None, dev)
+        _need(block_tables, "block_tables", _I32, None, dev)
         entries = block_tables.numel()
     p = _PoolArrays(pools, dev, P)
-    remap = torch.empty(P, dtype=_I32, device=dev)
-    live = torch.empty(1, dtype=_I32, device=dev)
+    remap = torch.empty_like(refcounts)
+    live = refcounts.new_empty(1)
     nws = 2 * (P // 2 + 1) + 1
-    ws = torch.empty(nws, dtype=_I32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("gdn_compact_pages", refcounts.data_ptr(), P,
-                  block_tables.data_ptr() if entries else None, entries, remap.data_ptr(),
-                  live.data_ptr(), p.ptrs, p.bytes, p.pitch, p.count, ws.data_ptr(), 4 * nws,
-                  _stream_handle(dev))
+    ws = refcounts.new_empty(nws)
+    _call(dev, "gdn_compact_pages", refcounts.data_ptr(), P,
+          block_tables.data_ptr() if entries else None, entries, remap.data_ptr(),
+          live.data_ptr(), p.ptrs, p.bytes, p.pitch, p.count, ws.data_ptr(), 4 * nws)
     return remap, live
