@@ -38,7 +38,8 @@ struct Pools {
 // A CTA takes one column (the same bytes of every page), reads it from all sources into
 // registers, waits for all its threads, and writes it to all destinations.  No other CTA
 // touches that column, so sources that are destinations too (a permutation of beams, a
-// cycle) are read before they are overwritten, without a second buffer: 2 x bytes moved.
+// cycle) are read before they are overwritten, without a second buffer; a source with several
+// destinations is read from HBM once, since its readers are in one CTA.
 
 struct CopyArgs {
   Pools pools;
@@ -49,49 +50,87 @@ struct CopyArgs {
   int hash;                        // entries of the hash table, a power of two >= 2 n
 };
 
-template <typename U>
+// Pairs that write: both indices valid, different, and no later valid pair with the same
+// destination.  Up to 32 pairs live in every warp's registers (lane i: the i-th of them);
+// more go through a hash table of destinations into a list in shared memory.
+template <bool kFew> struct Pairs;
+
+template <> struct Pairs<true> {
+  int s, d, n;
+  __device__ Pairs(const CopyArgs& p, int32_t*) {
+    const int lane = threadIdx.x % 32, P = p.pools.num_pages;
+    s = lane < p.n ? p.src[lane] : -1;
+    d = lane < p.n ? p.dst[lane] : -1;
+    const bool valid = s >= 0 && d >= 0 && s < P && d < P;
+    const bool beyond = s >= 0 && d >= 0 && !valid;
+    const uint32_t same = __match_any_sync(0xffffffffu, valid ? d : -1 - lane);
+    const uint32_t on = __ballot_sync(0xffffffffu, valid && s != d && (same >> lane) == 1);
+    const int bad = __popc(__ballot_sync(0xffffffffu, beyond));
+    if (bad && p.bad && blockIdx.x == 0 && threadIdx.x == 0) atomicAdd(p.bad, bad);
+    n = __popc(on);
+    const int from = lane < n ? __fns(on, 0, lane + 1) : 0;
+    s = __shfl_sync(0xffffffffu, s, from);
+    d = __shfl_sync(0xffffffffu, d, from);
+  }
+  __device__ int src(int i) const { return __shfl_sync(0xffffffffu, s, i & 31); }
+  __device__ int dst(int i) const { return __shfl_sync(0xffffffffu, d, i & 31); }
+};
+
+template <> struct Pairs<false> {
+  const int32_t* list;             // [2 n]: source, destination
+  int n;
+  __device__ Pairs(const CopyArgs& p, int32_t* smem) {
+    int32_t* key = smem;           // [hash] destination of an entry
+    int32_t* last = smem + p.hash; // [hash] its last pair
+    int32_t* out = smem + 2 * p.hash;
+    __shared__ int active, bad;
+    const int tid = threadIdx.x, P = p.pools.num_pages;
+    for (int i = tid; i < p.hash; i += kThreads) {
+      key[i] = -1;
+      last[i] = -1;
+    }
+    if (tid == 0) active = bad = 0;
+    __syncthreads();
+    auto slot_of = [&](int d) {
+      uint32_t at = static_cast<uint32_t>(d) * 2654435761u & (p.hash - 1);
+      while (true) {               // at most n of >= 2 n entries are taken
+        const int k = atomicCAS(&key[at], -1, d);
+        if (k == -1 || k == d) return at;
+        at = (at + 1) & (p.hash - 1);
+      }
+    };
+    for (int i = tid; i < p.n; i += kThreads) {
+      const int s = p.src[i], d = p.dst[i];
+      if (s < 0 || d < 0) continue;
+      if (s >= P || d >= P) {
+        atomicAdd(&bad, 1);
+        continue;
+      }
+      atomicMax(&last[slot_of(d)], i);
+    }
+    __syncthreads();
+    for (int i = tid; i < p.n; i += kThreads) {
+      const int s = p.src[i], d = p.dst[i];
+      if (s < 0 || d < 0 || s >= P || d >= P || s == d) continue;
+      if (last[slot_of(d)] != i) continue;
+      const int at = atomicAdd(&active, 1);
+      out[2 * at] = s;
+      out[2 * at + 1] = d;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && tid == 0 && p.bad && bad) atomicAdd(p.bad, bad);
+    list = out;
+    n = active;
+  }
+  __device__ int src(int i) const { return list[2 * min(i, n - 1)]; }
+  __device__ int dst(int i) const { return list[2 * min(i, n - 1) + 1]; }
+};
+
+template <typename U, bool kFew>
 __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyArgs p) {
   extern __shared__ int32_t smem[];
-  int32_t* key = smem;                    // [hash] dst of an entry
-  int32_t* last = smem + p.hash;          // [hash] its last pair
-  int32_t* list = smem + 2 * p.hash;      // [2 n] active pairs: src, dst
-  __shared__ int active, bad;
-  const int tid = threadIdx.x, P = p.pools.num_pages;
-  for (int i = tid; i < p.hash; i += kThreads) {
-    key[i] = -1;
-    last[i] = -1;
-  }
-  if (tid == 0) active = bad = 0;
-  __syncthreads();
-  auto slot_of = [&](int d) {
-    uint32_t at = static_cast<uint32_t>(d) * 2654435761u & (p.hash - 1);
-    while (true) {                        // at most n of >= 2 n entries are taken
-      const int k = atomicCAS(&key[at], -1, d);
-      if (k == -1 || k == d) return at;
-      at = (at + 1) & (p.hash - 1);
-    }
-  };
-  for (int i = tid; i < p.n; i += kThreads) {
-    const int s = p.src[i], d = p.dst[i];
-    if (s < 0 || d < 0) continue;
-    if (s >= P || d >= P) {
-      atomicAdd(&bad, 1);
-      continue;
-    }
-    atomicMax(&last[slot_of(d)], i);
-  }
-  __syncthreads();
-  for (int i = tid; i < p.n; i += kThreads) {
-    const int s = p.src[i], d = p.dst[i];
-    if (s < 0 || d < 0 || s >= P || d >= P || s == d) continue;
-    if (last[slot_of(d)] != i) continue;
-    const int at = atomicAdd(&active, 1);
-    list[2 * at] = s;
-    list[2 * at + 1] = d;
-  }
-  __syncthreads();
-  if (blockIdx.x == 0 && tid == 0 && p.bad && bad) atomicAdd(p.bad, bad);
-  const int n = active;
+  const Pairs<kFew> pairs(p, smem);
+  const int n = pairs.n, tid = threadIdx.x;
   if (n == 0) return;
   // vectors of one page per column: as many as the registers hold, fewer when that would
   // leave CTAs without a column
@@ -99,27 +138,31 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
   while ((2 << shift) * n <= kThreads * kVecs) ++shift;
   long long total = 0;
   for (int i = 0; i < p.pools.count; ++i) total += p.pools.bytes[i] / static_cast<int>(sizeof(U));
-  while (shift > 5 && (total >> shift) < gridDim.x) --shift;
+  while (shift > 5 && (total >> shift) * 2 <= gridDim.x) --shift;
+  const int held = ((n << shift) + kThreads - 1) / kThreads;   // vectors of a thread, <= kVecs
   long long item = blockIdx.x;
   for (int pool = 0; pool < p.pools.count; ++pool) {
     const long long vecs = p.pools.bytes[pool] / static_cast<int>(sizeof(U));
-    const long long cols = (vecs + (1ll << shift) - 1) >> shift;
+    const long long cols = (vecs + (1ll << shift) - 1) >> shift, pitch = p.pools.pitch[pool];
+    char* base = p.pools.base[pool];
     for (; item < cols; item += gridDim.x) {
       U v[kVecs];
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
+        if (k >= held) break;
         const int f = tid + k * kThreads, i = f >> shift;
         const long long at = (item << shift) + (f & ((1 << shift) - 1));
-        if (i < n && at < vecs)
-          v[k] = reinterpret_cast<const U*>(p.pools.base[pool] + list[2 * i] * p.pools.pitch[pool])[at];
+        const int page = pairs.src(i);
+        if (i < n && at < vecs) v[k] = reinterpret_cast<const U*>(base + page * pitch)[at];
       }
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
+        if (k >= held) break;
         const int f = tid + k * kThreads, i = f >> shift;
         const long long at = (item << shift) + (f & ((1 << shift) - 1));
-        if (i < n && at < vecs)
-          reinterpret_cast<U*>(p.pools.base[pool] + list[2 * i + 1] * p.pools.pitch[pool])[at] = v[k];
+        const int page = pairs.dst(i);
+        if (i < n && at < vecs) reinterpret_cast<U*>(base + page * pitch)[at] = v[k];
       }
     }
     item -= cols;
@@ -137,10 +180,19 @@ struct MoveArgs {
   const int32_t* dst;
   const int32_t* count;            // device count of pairs, or null: n
   int n;
+  int32_t* tables;                 // entries to rewrite through remap, or null
+  const int32_t* remap;            // [num_pages]
+  long long entries;
 };
 
 template <typename U>
 __global__ void __launch_bounds__(kThreads) move_pages_kernel(const __grid_constant__ MoveArgs p) {
+  grid_wait();                     // the plan is the kernel before
+  const long long step = static_cast<long long>(gridDim.x) * kThreads;
+  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < p.entries; i += step) {
+    const int page = p.tables[i];
+    if (page >= 0 && page < p.pools.num_pages) p.tables[i] = p.remap[page];
+  }
   const long long n = p.count ? *p.count : p.n;
   long long item = blockIdx.x;
   for (int pool = 0; pool < p.pools.count; ++pool) {
@@ -212,16 +264,37 @@ __device__ void assign_free(int32_t* refcounts, int P, int n, int32_t* row_of, W
     needed += total;
   }
   __syncthreads();
+  // four neighbouring pages per thread and round, the next round's counts on their way
   int found = 0;
-  for (int p0 = 0; p0 < P && found < needed; p0 += kPlanThreads) {
-    const int page = p0 + threadIdx.x;
-    const int f = page < P && refcounts[page] <= 0;
-    const int at = found + block_scan(f, total);
-    if (f && at < needed) {
-      refcounts[page] = 1;
-      give(row_of[at], page);
+  auto load = [&](int p0, int (&c)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int page = p0 + 4 * threadIdx.x + u;
+      c[u] = page < P ? refcounts[page] : 1;
     }
+  };
+  int c[4];
+  load(0, c);
+  for (int p0 = 0; p0 < P && found < needed; p0 += 4 * kPlanThreads) {
+    int next[4];
+    load(p0 + 4 * kPlanThreads, next);
+    int f = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f += c[u] <= 0;
+    int at = found + block_scan(f, total);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (c[u] <= 0) {
+        if (at < needed) {
+          const int page = p0 + 4 * threadIdx.x + u;
+          refcounts[page] = 1;
+          give(row_of[at], page);
+        }
+        ++at;
+      }
     found += total;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[u] = next[u];
   }
   for (int k = found + threadIdx.x; k < needed; k += kPlanThreads) give(row_of[k], -1);
 }
@@ -266,7 +339,8 @@ struct ForkArgs {
 };
 
 // CTA r: the references of input row r, and output row r.
-__global__ void __launch_bounds__(kThreads) fork_rows_kernel(ForkArgs p) {
+__global__ void __launch_bounds__(kThreads) fork_rows_kernel(const __grid_constant__ ForkArgs p) {
+  grid_trigger();
   const int r = blockIdx.x, tid = threadIdx.x;
   __shared__ int count, earlier;
   if (tid == 0) count = earlier = 0;
@@ -309,7 +383,9 @@ __global__ void __launch_bounds__(kThreads) fork_rows_kernel(ForkArgs p) {
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs p) {
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ ForkArgs p) {
+  grid_trigger();
+  grid_wait();                     // the rows' references are counted
   assign_free(p.refcounts, p.P, p.rows_out, p.row_of, [&](int i) { return p.src[i] >= 0; },
               [&](int i, int page) {
                 p.dst[i] = page;
@@ -328,42 +404,91 @@ struct CompactArgs {
   int P;
 };
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs p) {
-  int c = 0, live;
-  for (int i = threadIdx.x; i < p.P; i += kPlanThreads) c += p.refcounts[i] > 0;
-  block_scan(c, live);
-  int movers = 0, holes = 0, total;
-  for (int i0 = 0; i0 < p.P; i0 += kPlanThreads) {
-    const int i = i0 + threadIdx.x;
-    const bool in = i < p.P, on = in && p.refcounts[i] > 0;
-    const int mv = on && i >= live, ho = in && !on && i < live;
-    const int am = movers + block_scan(mv, total);
-    movers += total;
-    const int ah = holes + block_scan(ho, total);
-    holes += total;
-    if (mv) p.src[am] = i;
-    if (ho) p.dst[ah] = i;
-    if (in) p.remap[i] = on ? i : -1;
+// Each thread looks after a run of neighbouring pages, four at a time.  With before(i) the
+// live pages before page i and L all of them, a free page i < L is hole number
+// i - before(i), and a live page i >= L is mover number before(i) - before(L); there are
+// L - before(L) of either.  The k-th of each are paired through shared memory, or through the
+// workspace where there are more than it holds.
+constexpr int kPaired = 4096;
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactArgs p) {
+  __shared__ int before_live, hole[kPaired];
+  grid_trigger();
+  const int groups = (p.P + 3) / 4, run = (groups + kPlanThreads - 1) / kPlanThreads;
+  const int g0 = min(static_cast<int>(threadIdx.x) * run, groups), g1 = min(g0 + run, groups);
+  const bool wide = (reinterpret_cast<uintptr_t>(p.refcounts) & 15) == 0;
+  auto counts = [&](int g) {       // of pages 4 g ... 4 g + 3; 0 past the last
+    if (wide && 4 * g + 4 <= p.P) return reinterpret_cast<const int4*>(p.refcounts)[g];
+    int4 c = make_int4(0, 0, 0, 0);
+    if (4 * g < p.P) c.x = p.refcounts[4 * g];
+    if (4 * g + 1 < p.P) c.y = p.refcounts[4 * g + 1];
+    if (4 * g + 2 < p.P) c.z = p.refcounts[4 * g + 2];
+    if (4 * g + 3 < p.P) c.w = p.refcounts[4 * g + 3];
+    return c;
+  };
+  int mine = 0, live;
+#pragma unroll 2
+  for (int g = g0; g < g1; ++g) {
+    const int4 c = counts(g);
+    mine += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
+  }
+  const int first = block_scan(mine, live);
+  if (threadIdx.x == 0) before_live = live;                  // where all pages are live
+  __syncthreads();
+  if (4 * g0 <= live && live < 4 * g1 && live < p.P) {
+    int n = first;
+    for (int i = 4 * g0; i < live; ++i) n += p.refcounts[i] > 0;
+    before_live = n;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < movers; k += kPlanThreads) {
-    const int s = p.src[k], d = p.dst[k];
-    p.remap[s] = d;
-    p.refcounts[d] = p.refcounts[s];
-    p.refcounts[s] = 0;
+  const int kept = before_live, movers = live - kept;
+  int before = first;
+#pragma unroll 2
+  for (int g = g0; g < g1; ++g) {
+    const int4 c = counts(g);
+    const int* cs = &c.x;
+    int to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = 4 * g + u;
+      const bool on = cs[u] > 0;
+      to[u] = on ? i : -1;
+      if (!on && i < live) {       // live <= P: the padding is no hole
+        const int k = i - before;
+        p.dst[k] = i;
+        if (k < kPaired) hole[k] = i;
+      }
+      before += on;
+    }
+    if (wide && 4 * g + 4 <= p.P && (reinterpret_cast<uintptr_t>(p.remap) & 15) == 0) {
+      reinterpret_cast<int4*>(p.remap)[g] = make_int4(to[0], to[1], to[2], to[3]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (4 * g + u < p.P) p.remap[4 * g + u] = to[u];
+    }
+  }
+  __syncthreads();
+  // the movers: only counts of pages before `live` change here, and those are not read
+  before = first;
+  for (int g = max(g0, live / 4); g < g1; ++g) {
+    const int4 c = counts(g);
+    const int* cs = &c.x;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = 4 * g + u;
+      if (i == live) before = kept;
+      if (i < live || cs[u] <= 0) continue;
+      const int k = before++ - kept, d = k < kPaired ? hole[k] : p.dst[k];
+      p.src[k] = i;
+      p.remap[i] = d;
+      p.refcounts[d] = cs[u];
+      p.refcounts[i] = 0;
+    }
   }
   if (threadIdx.x == 0) {
     *p.live = live;
     *p.count = movers;
-  }
-}
-
-__global__ void __launch_bounds__(kThreads)
-remap_tables_kernel(int32_t* tables, long long n, const int32_t* remap, int P) {
-  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n; i += step) {
-    const int page = tables[i];
-    if (page >= 0 && page < P) tables[i] = remap[page];
   }
 }
 
@@ -402,19 +527,21 @@ int check_pools(void* const* pools, const int64_t* bytes, const int64_t* pitch, 
   return GDN_OK;
 }
 
-// enough CTAs for the vectors to move, at most two per SM
-unsigned grid_for(const Pools& pools, int unit, long long pairs) {
+// CTAs for `pairs` pages to move: two per SM with as few vectors per thread as that leaves,
+// and past full registers one per kVecs vectors of its threads, up to `most` per SM.
+unsigned grid_for(const Pools& pools, int unit, long long pairs, int most) {
   long long vecs = 0;
   for (int i = 0; i < pools.count; ++i) vecs += pools.bytes[i] / unit;
-  long long ctas = (vecs * pairs + kThreads - 1) / kThreads;
-  return static_cast<unsigned>(ctas < 1 ? 1 : ctas > 2 * 148 ? 2 * 148 : ctas);
+  const long long thin = (vecs * pairs + kThreads - 1) / kThreads;
+  const long long full = (thin + kVecs - 1) / kVecs;
+  const long long two = 2 * kSMs, ctas = full > two ? full : thin < two ? thin : two;
+  return static_cast<unsigned>(ctas < 1 ? 1 : ctas > 1ll * most * kSMs ? most * kSMs : ctas);
 }
 
 cudaError_t launch_moves(const MoveArgs& a, int unit, unsigned grid, cudaStream_t st) {
-  if (unit == 16) move_pages_kernel<uint4><<<grid, kThreads, 0, st>>>(a);
-  else if (unit == 4) move_pages_kernel<uint32_t><<<grid, kThreads, 0, st>>>(a);
-  else move_pages_kernel<uint8_t><<<grid, kThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  if (unit == 16) return launch_after(move_pages_kernel<uint4>, dim3(grid), dim3(kThreads), 0, st, a);
+  if (unit == 4) return launch_after(move_pages_kernel<uint32_t>, dim3(grid), dim3(kThreads), 0, st, a);
+  return launch_after(move_pages_kernel<uint8_t>, dim3(grid), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
@@ -437,10 +564,11 @@ int gdn_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t*
   a.dst = dst;
   a.bad = bad_index_count;
   a.n = n;
-  a.hash = 64;
-  while (a.hash < 2 * n) a.hash *= 2;
-  const size_t smem = (2 * static_cast<size_t>(a.hash) + 2 * static_cast<size_t>(n)) * 4;
-  const unsigned grid = grid_for(a.pools, unit, n);
+  const bool few = n <= 32;
+  a.hash = few ? 0 : 64;
+  while (a.hash && a.hash < 2 * n) a.hash *= 2;
+  const size_t smem = few ? 0 : (2 * static_cast<size_t>(a.hash) + 2 * static_cast<size_t>(n)) * 4;
+  const unsigned grid = grid_for(a.pools, unit, n, 32);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto kernel) {
     if (smem > 48 * 1024 &&
@@ -450,8 +578,9 @@ int gdn_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t*
     kernel<<<grid, kThreads, smem, st>>>(a);
     return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
   };
-  return unit == 16 ? go(copy_pages_kernel<uint4>)
-                    : unit == 4 ? go(copy_pages_kernel<uint32_t>) : go(copy_pages_kernel<uint8_t>);
+  if (unit == 16) return few ? go(copy_pages_kernel<uint4, true>) : go(copy_pages_kernel<uint4, false>);
+  if (unit == 4) return few ? go(copy_pages_kernel<uint32_t, true>) : go(copy_pages_kernel<uint32_t, false>);
+  return few ? go(copy_pages_kernel<uint8_t, true>) : go(copy_pages_kernel<uint8_t, false>);
 }
 
 int gdn_alloc_pages(int32_t* refcounts, int num_pages, const uint8_t* need, int n, int32_t* pages,
@@ -474,7 +603,7 @@ int gdn_free_pages(int32_t* refcounts, int num_pages, const int32_t* pages, int6
   if (!aligned(refcounts, 4) || !aligned(pages, 4) || !aligned(bad_index_count, 4))
     return GDN_ERR_ALIGN;
   const int64_t ctas = (n + kThreads - 1) / kThreads;
-  free_pages_kernel<<<static_cast<unsigned>(ctas > 148 * 8 ? 148 * 8 : ctas), kThreads, 0,
+  free_pages_kernel<<<static_cast<unsigned>(ctas > kSMs * 8 ? kSMs * 8 : ctas), kThreads, 0,
                       static_cast<cudaStream_t>(stream)>>>(refcounts, num_pages, pages, n,
                                                            bad_index_count);
   return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
@@ -523,13 +652,13 @@ int gdn_fork_pages(const int32_t* block_tables, int64_t table_stride, const int3
   fork_rows_kernel<<<rows_in > rows_out ? rows_in : rows_out, kThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
   if (rows_out == 0) return GDN_OK;
-  fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
+  if (launch_after(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p) != cudaSuccess)
+    return GDN_ERR_LAUNCH;
   if (num_pools == 0) return GDN_OK;
   m.src = p.src;
   m.dst = p.dst;
   m.n = rows_out;
-  return launch_moves(m, unit, grid_for(m.pools, unit, rows_out), st) == cudaSuccess ? GDN_OK
+  return launch_moves(m, unit, grid_for(m.pools, unit, rows_out, 8), st) == cudaSuccess ? GDN_OK
                                                                                      : GDN_ERR_LAUNCH;
 }
 
@@ -557,17 +686,17 @@ int gdn_compact_pages(int32_t* refcounts, int num_pages, int32_t* block_tables,
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
-  if (table_entries > 0) {
-    const int64_t ctas = (table_entries + kThreads - 1) / kThreads;
-    remap_tables_kernel<<<static_cast<unsigned>(ctas > 148 * 8 ? 148 * 8 : ctas), kThreads, 0, st>>>(
-        block_tables, table_entries, remap, num_pages);
-    if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
-  }
-  if (num_pools == 0) return GDN_OK;
+  if (num_pools == 0 && table_entries == 0) return GDN_OK;
+  m.tables = block_tables;
+  m.entries = table_entries;
+  m.remap = remap;
   m.src = p.src;
   m.dst = p.dst;
   m.count = p.count;
-  return launch_moves(m, unit, grid_for(m.pools, unit, static_cast<long long>(half)), st) == cudaSuccess
+  const unsigned grid = num_pools > 0 ? grid_for(m.pools, unit, static_cast<long long>(half), 8)
+                                      : static_cast<unsigned>(table_entries < 2 * kSMs * kThreads
+                                            ? (table_entries + kThreads - 1) / kThreads : 2 * kSMs);
+  return launch_moves(m, unit, grid, st) == cudaSuccess
              ? GDN_OK : GDN_ERR_LAUNCH;
 }
 
