@@ -35,12 +35,12 @@ struct AttnArgs {
   int32_t* bad;              // or null
   float* part_o;             // workspace [2 grid, heads of a row, D]: sums of p v
   float* part_ml;            // workspace [2 grid, heads of a row, 2]: their m and l
-  int4* cut;                 // workspace [grid]: the cut row that ends in this share, or none
+  int4* cut;                 // workspace: the cut rows, by row or by the share they end in
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // byte strides
   long long table_stride;
   float scale_log2;          // scale * log2(e): the softmax runs in base 2
   uint32_t page_mul, page_shift;
-  int B, HQ, HKV, group, tiles, grid, num_pages, page_size, width, window, sinks, twin;
+  int B, HQ, HKV, group, tiles, grid, num_pages, page_size, width, window, sinks, twin, by_row;
 };
 
 // One sequence's lengths: tokens held, tokens visible, whether the new token is in play.
@@ -49,10 +49,9 @@ struct Seq {
   bool append;
 };
 
-__device__ __forceinline__ Seq sequence(const AttnArgs& p, int b) {
+__device__ __forceinline__ Seq sequence(const AttnArgs& p, int n) {   // n: its seq_lens
   Seq s;
   const int cap = p.width * p.page_size;   // < 2^31, checked on the host
-  int n = p.lens[b];
   n = n < 0 ? 0 : n;
   s.append = p.k_new != nullptr && n > 0 && n <= cap;
   s.len = n > cap ? cap : n;
@@ -69,7 +68,8 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& p, int b) {
 // and many short ones all load the GPU evenly.  A CTA that has all of a row writes its
 // output; a row that is cut leaves partial sums (at most two per CTA: its first and its last
 // row), which attn_join_kernel adds up in a fixed order.  The cut depends on lens alone, so
-// no counters or flags have to be kept in memory.
+// no counters or flags have to be kept in memory.  In a call whose rows all are short
+// none is cut (cut == null): a row is then one unit of the line.
 
 constexpr int kWarps = 4;
 
@@ -85,8 +85,10 @@ template <int D> struct Shape {
   static constexpr int kResident = D == 256 ? 1 : 2;
 };
 
+// units of one of sequence b's rows in the line
 template <int kBlock> __device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
-  const int vis = sequence(p, b).vis;
+  if (!p.cut) return 1;
+  const int vis = sequence(p, p.lens[b]).vis;
   return vis > 0 ? (vis + kBlock - 1) / kBlock : 1;
 }
 
@@ -207,9 +209,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // registers.  p is rounded to the tensors' type for that product (its own sum l is not):
 // the rounding is that of the values it multiplies, at most half a step of each weight.
 //
-// Every warp streams its own 16-token tiles through its own ring of kStages buffers in
-// shared memory with asynchronous copies, so the main loop has no CTA barrier.  A tile's page
-// numbers are loaded one tile before its copies are issued.
+// Every warp streams its own tiles of 16 or 32 tokens through its own ring of kStages
+// buffers in shared memory with asynchronous copies, so the main loop has no CTA barrier.
+// A tile's page numbers are loaded one tile before its copies are issued, and the copies run
+// on into the share's next row, so a short row does not empty the pipeline.
 
 // A tile's row r has its 16-byte chunk c at r kRow + ((c ^ (r & 7)) << 4): the eight rows that a
 // matrix load touches lie in different banks.  Stages are aligned to rows, so stepping
@@ -223,8 +226,9 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   constexpr int MT = S::kTile / 16;                           // 16-token parts of a tile
   constexpr int kRows = 32 / CPR, kIters = S::kTile / kRows;  // rows a warp copies at a time
   constexpr uint32_t kAll = S::kTile == 32 ? 0xffffffffu : 0xffffu;
-  constexpr int kPad = D + 4;                                 // floats of a head in the merge
-  static_assert(kHeads * kPad * 4 <= S::kWarpBytes, "the merge reuses the ring");
+  constexpr int kPad = kHeads * (D + 4) * 4 <= 2 * S::kHalf ? D + 4 : D;   // floats of a head in the merge
+  static_assert(kHeads * kPad * 4 <= 2 * S::kHalf, "the merge reuses a stage");
+  static_assert(S::kStages == 3, "two tiles ahead of the one being multiplied");
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -234,9 +238,8 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   const Share share = my_share<S::kBlock>(p);
   const int rows = p.HKV * p.tiles;                           // rows of one sequence
   long long at = share.start, before = share.before;
-  int b = share.b;
   if (at == share.end) {
-    if (tid == 0 && p.cut) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && p.cut && !p.by_row) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 
@@ -246,121 +249,166 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   const uint32_t k_at = (lane % 16) * S::kRow + (((lane >> 4) ^ (lane & 7)) << 4);
   const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * S::kRow + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
-  while (at < share.end) {
-    const Seq s = sequence(p, b);
-    const int nb = s.vis > 0 ? (s.vis + S::kBlock - 1) / S::kBlock : 1;
-    const long long in_seq = at - before * rows;
-    const int row = static_cast<int>(in_seq / nb), k0 = static_cast<int>(in_seq % nb);
-    const long long left = share.end - at;
-    const int k1 = left < nb - k0 ? k0 + static_cast<int>(left) : nb;
-    const int g = row / p.tiles, tile = row % p.tiles;
-    const int head0 = g * p.group + tile * kHeads, heads = min(kHeads, p.group - tile * kHeads);
-    const int32_t* table = p.tables + b * p.table_stride;
-    const long long new_row = (static_cast<long long>(b) * p.HKV + g) * D * 2;
-    const char* kbase = p.k + g * p.k_head;
-    const char* vbase = p.v + g * p.v_head;
-    const bool counts = row == 0 && p.bad != nullptr;
-    if (counts && tid == 0 && k0 == 0 && p.lens[b] > s.len) atomicAdd(p.bad, 1);
-    if (at == share.start && tid == 0 && p.cut) {
-      const long long first = before * rows + static_cast<long long>(row) * nb;
-      const int c0 = static_cast<int>(share_of(first, share.total, share.count));
-      p.cut[blockIdx.x] = make_int4(k0 > 0 && k1 == nb ? b : -1, row, c0,
-                                    first > share_start(c0, share.total, share.count));
-    }
+  // The copies run ahead of the products, into the share's next row as well: `f` is the row
+  // being copied, `row` the one being multiplied, `next` what f will be when row gets there.
+  struct Row {
+    int b, row, blocks, whole;
+  };
+  Row row = {}, next = {};
+  Seq f = {};
+  int f_b = share.b, f_row = 0, f_k = 0, f_k1 = 0, page = -1;
+  int len_next = 0;                       // tokens of sequence f_b + 1, loaded early
+  bool ahead_row = false;                 // f is `next`, not `row`
+  int ahead = 0, put = 0;                 // tiles copied ahead; the stage the next one goes to
+  uint32_t mask[2] = {0u, 0u};            // tokens seen of the tiles copied ahead
 
-    // lane i looks after token i of a tile (all 32, or twice 16): its page number, its place
-    auto token_of = [&](int k) {
-      const int j = (k * kWarps + warp) * S::kTile + (lane & (S::kTile - 1));
-      return j < s.vis ? (j < p.sinks ? j : j + s.shift) : -1;
-    };
-    auto page_of = [&](int k) {
-      const int tok = k < k1 ? token_of(k) : -1;
-      return tok < 0 ? -1 : __ldg(table + div_by(tok, p.page_mul, p.page_shift));
-    };
-    // whether no visible token before tok lies in its page
-    auto first_in_page = [&](int tok, int off) {
-      if (off == 0) return true;
-      return s.shift > 0 && tok == p.sinks + s.shift &&
-             (p.sinks == 0 || (p.sinks - 1) / p.page_size != tok / p.page_size);
-    };
-    // issue the copies of block k's tile into ring stage st; returns the tokens seen
-    auto fetch = [&](int k, int st, int page) -> uint32_t {
-      const int tok = token_of(k);
-      const int off = tok < 0 ? 0 : tok - static_cast<int>(div_by(tok, p.page_mul, p.page_shift)) * p.page_size;
-      const bool is_new = s.append && tok == s.len - 1;
-      const bool in_cache = tok >= 0 && page >= 0 && page < p.num_pages;
-      if (counts && lane < S::kTile && tok >= 0 && page >= p.num_pages && first_in_page(tok, off))
-        atomicAdd(p.bad, 1);
-      const uint32_t mask = __ballot_sync(0xffffffffu, in_cache || is_new) & kAll;
-      const bool any_new = __any_sync(0xffffffffu, is_new);
-      // this lane's token's row, relative to the head's first row
-      long long ko = in_cache ? page * p.k_page + off * p.k_tok : 0;
-      long long vo = in_cache ? page * p.v_page + off * p.v_tok : 0;
-      if (is_new) {
-        ko = reinterpret_cast<const char*>(p.k_new) + new_row - kbase;
-        vo = reinterpret_cast<const char*>(p.v_new) + new_row - vbase;
+  // lane i looks after token i of a tile (all 32, or twice 16): its page number, its place
+  auto token_of = [&](int k) {
+    const int j = (k * kWarps + warp) * S::kTile + (lane & (S::kTile - 1));
+    return j < f.vis ? (j < p.sinks ? j : j + f.shift) : -1;
+  };
+  auto page_of = [&](int k) {
+    const int tok = token_of(k);
+    return tok < 0 ? -1 : __ldg(p.tables + f_b * p.table_stride + div_by(tok, p.page_mul, p.page_shift));
+  };
+  // Turns to the row at line position `at` (of sequence f_b, whose tokens are `len`).
+  auto open = [&](Row& r, int len) {
+    f = sequence(p, len);
+    const int nb = f.vis > 0 ? (f.vis + S::kBlock - 1) / S::kBlock : 1;
+    const long long in_seq = at - before * rows, left = share.end - at;
+    const int units = p.cut ? nb : 1;
+    f_row = static_cast<int>(in_seq / units);
+    f_k = static_cast<int>(in_seq - static_cast<long long>(f_row) * units);
+    f_k1 = !p.cut || left >= nb - f_k ? nb : f_k + static_cast<int>(left);
+    r.b = f_b;
+    r.row = f_row;
+    r.blocks = f_k1 - f_k;
+    r.whole = f_k == 0 && f_k1 == nb;
+    page = page_of(f_k);
+    if (tid == 0) {
+      if (f_row == 0 && f_k == 0 && p.bad != nullptr && len > f.len) atomicAdd(p.bad, 1);
+      if (p.cut && (p.by_row ? f_k1 == nb : at == share.start)) {
+        const long long first = before * rows + static_cast<long long>(f_row) * nb;
+        const int c0 = static_cast<int>(share_of(first, share.total, share.count));
+        const int late = first > share_start(c0, share.total, share.count);   // c0's last row
+        p.cut[p.by_row ? static_cast<long long>(f_b) * rows + f_row : blockIdx.x] =
+            make_int4(f_k > 0 && f_k1 == nb ? f_b : -1, f_row, c0, 2 * blockIdx.x + late);
       }
-      const uint32_t dst = ring + st * 2 * S::kHalf + copy_at;
-      const char* kc = kbase + copy_c * 16;
-      const char* vc = vbase + copy_c * 16;
-      if (mask == kAll && p.twin && !any_new) {               // nearly always
-#pragma unroll
-        for (int i = 0; i < kIters; ++i) {
-          const long long o = __shfl_sync(0xffffffffu, ko, copy_r + i * kRows);
-          const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
-          copy16_async(d, kc + o, true);
-          copy16_async(d + S::kHalf, vc + o, true);
-        }
-      } else {
-#pragma unroll 2
-        for (int i = 0; i < kIters; ++i) {
-          const int r = copy_r + i * kRows;
-          const long long o = __shfl_sync(0xffffffffu, ko, r), w = __shfl_sync(0xffffffffu, vo, r);
-          const bool ok = (mask >> r) & 1;
-          const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
-          copy16_async(d, kc + o, ok);
-          copy16_async(d + S::kHalf, vc + w, ok);
-        }
-      }
-      return mask;
-    };
-
-    uint32_t mask[S::kStages - 1];
-    int page = page_of(k0);
-#pragma unroll
-    for (int st = 0; st < S::kStages - 1; ++st) {
-      mask[st] = 0;
-      const int next = page_of(k0 + st + 1);
-      if (k0 + st < k1) mask[st] = fetch(k0 + st, st, page);
-      page = next;
-      copy_commit();
     }
     // the new token's rows go into the cache once: by the first tile's owner of the last block
-    if (s.append && tile == 0 && k1 == nb) {
-      const int tok = s.len - 1, pi = tok / p.page_size, pg = table[pi];
-      if (pg >= 0 && pg < p.num_pages && tid < 2 * CPR) {
+    const int g = f_row / p.tiles;
+    if (f.append && f_row == g * p.tiles && f_k1 == nb && tid < 2 * CPR) {
+      const int tok = f.len - 1, pi = tok / p.page_size, pg = p.tables[f_b * p.table_stride + pi];
+      if (pg >= 0 && pg < p.num_pages) {
         const int c = tid % CPR, of = tok - pi * p.page_size;
-        const char* src = reinterpret_cast<const char*>(tid < CPR ? p.k_new : p.v_new) + new_row;
+        const long long from = (static_cast<long long>(f_b) * p.HKV + g) * (D * 2);
+        const char* src = reinterpret_cast<const char*>(tid < CPR ? p.k_new : p.v_new) + from;
         char* dst = tid < CPR ? p.k + g * p.k_head + pg * p.k_page + of * p.k_tok
                               : p.v + g * p.v_head + pg * p.v_page + of * p.v_tok;
         *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(src + c * 16);
       }
     }
-    // queries as the right operand: head lane / 4 (+ 8 per further group), two dims a register
-    uint32_t qf[NG][KS][2];
+    // where the line goes on after this row
+    at += p.cut ? f_k1 - f_k : 1;
+    if (f_row == rows - 1 && f_k1 == nb) {
+      before += units;
+      if (f_b + 1 < p.B) len_next = p.lens[f_b + 1];
+    }
+  };
+  // whether no visible token before tok lies in its page
+  auto first_in_page = [&](int tok, int off) {
+    if (off == 0) return true;
+    return f.shift > 0 && tok == p.sinks + f.shift &&
+           (p.sinks == 0 || (p.sinks - 1) / p.page_size != tok / p.page_size);
+  };
+  // issue the copies of f's next tile, if there is one, and look up the pages of the one after
+  auto fetch = [&]() {
+    if (f_k == f_k1) return;
+    const int tok = token_of(f_k);
+    const int off = tok < 0 ? 0 : tok - static_cast<int>(div_by(tok, p.page_mul, p.page_shift)) * p.page_size;
+    const bool is_new = f.append && tok == f.len - 1;
+    const bool in_cache = tok >= 0 && page >= 0 && page < p.num_pages;
+    if (f_row == 0 && p.bad != nullptr && lane < S::kTile && tok >= 0 && page >= p.num_pages &&
+        first_in_page(tok, off))
+      atomicAdd(p.bad, 1);
+    const uint32_t seen = __ballot_sync(0xffffffffu, in_cache || is_new) & kAll;
+    const bool any_new = __any_sync(0xffffffffu, is_new);
+    // this lane's token's row in the caches
+    const int g = f_row / p.tiles;
+    long long ko = in_cache ? g * p.k_head + page * p.k_page + off * p.k_tok : 0;
+    const uint32_t dst = ring + put * 2 * S::kHalf + copy_at;
+    const char* kc = p.k + copy_c * 16;
+    if (seen == kAll && p.twin && !any_new) {                 // nearly always
+      const char* vc = p.v + copy_c * 16;
+#pragma unroll
+      for (int i = 0; i < kIters; ++i) {
+        const long long o = __shfl_sync(0xffffffffu, ko, copy_r + i * kRows);
+        const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
+        copy16_async(d, kc + o, true);
+        copy16_async(d + S::kHalf, vc + o, true);
+      }
+    } else {
+      long long vo = in_cache ? g * p.v_head + page * p.v_page + off * p.v_tok : 0;
+      const char* vc = p.v + copy_c * 16;
+      if (is_new) {
+        const long long from = (static_cast<long long>(f_b) * p.HKV + g) * (D * 2);
+        ko = reinterpret_cast<const char*>(p.k_new) + from - p.k;
+        vo = reinterpret_cast<const char*>(p.v_new) + from - p.v;
+      }
+#pragma unroll 2
+      for (int i = 0; i < kIters; ++i) {
+        const int r = copy_r + i * kRows;
+        const long long o = __shfl_sync(0xffffffffu, ko, r), w = __shfl_sync(0xffffffffu, vo, r);
+        const bool ok = (seen >> r) & 1;
+        const uint32_t d = (dst ^ ((i * kRows & 7) << 4)) + i * kRows * S::kRow;
+        copy16_async(d, kc + o, ok);
+        copy16_async(d + S::kHalf, vc + w, ok);
+      }
+    }
+    copy_commit();
+    if (ahead == 0) mask[0] = seen;
+    else mask[1] = seen;
+    ++ahead;
+    put = put + 1 == S::kStages ? 0 : put + 1;
+    if (++f_k < f_k1) page = page_of(f_k);
+  };
+  // turn to the share's next row once the present one is copied and multiplication is there
+  auto advance = [&]() {
+    if (f_k == f_k1 && !ahead_row && at < share.end) {
+      const bool same = f_row + 1 < rows;                     // the sequence has more rows
+      f_b += same ? 0 : 1;
+      open(next, same ? p.lens[f_b] : len_next);
+      ahead_row = true;
+    }
+  };
+  // queries as the right operand: head lane / 4 (+ 8 per further group), two dims a register
+  uint32_t qf[NG][KS][2];
+  auto load_queries = [&]() {
+    const int g = row.row / p.tiles, tile = row.row - g * p.tiles;
+    const int heads = min(kHeads, p.group - tile * kHeads);
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const int h = n * 8 + lane / 4;
       const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q) +
-                          (static_cast<long long>(b) * p.HQ + head0 + (h < heads ? h : 0)) * (D / 2);
+                          (static_cast<long long>(row.b) * p.HQ + g * p.group + tile * kHeads +
+                           (h < heads ? h : 0)) * (D / 2);
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         qf[n][i][0] = h < heads ? __ldg(q + i * 8 + lane % 4) : 0u;
         qf[n][i][1] = h < heads ? __ldg(q + i * 8 + 4 + lane % 4) : 0u;
       }
     }
+  };
 
-    float o[NG][KS][4], m[NG][2], l[NG][2];
+  open(row, p.lens[f_b]);
+  load_queries();
+  fetch();
+  advance();
+  fetch();
+  advance();
+
+  float o[NG][KS][4], m[NG][2], l[NG][2];
+  auto clear = [&]() {
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -370,107 +418,113 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
     }
-
-    int st = 0;
-    for (int k = k0; k < k1; ++k) {
-      copy_wait<S::kStages - 2>();
-      __syncwarp();
-      const uint32_t buf = ring + st * 2 * S::kHalf;
-      const uint32_t seen = mask[0];
-      float y[MT][NG][4];
+  };
+  clear();
+  bool first_row = true;
+  int st = 0;
+  while (true) {
+    if (ahead == 2) copy_wait<1>();
+    else copy_wait<0>();
+    __syncwarp();
+    const uint32_t buf = ring + st * 2 * S::kHalf;
+    const uint32_t seen = mask[0];
+    float y[MT][NG][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float x[NG][2][4];                  // two chains of products
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t a[4];
+        load_matrices(a, (buf + k_at + t * 16 * S::kRow) ^ (i * 32));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+      }
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[t][n][j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
+    }
+    if (seen != kAll) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          if (!((seen >> (t * 16 + lane / 4)) & 1)) y[t][n][0] = y[t][n][1] = -INFINITY;
+          if (!((seen >> (t * 16 + lane / 4 + 8)) & 1)) y[t][n][2] = y[t][n][3] = -INFINITY;
+        }
+    }
+    uint32_t pb[MT][NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        float x[NG][2][4];                // two chains of products
+        t0 = fmaxf(t0, fmaxf(y[t][n][0], y[t][n][2]));
+        t1 = fmaxf(t1, fmaxf(y[t][n][1], y[t][n][3]));
+      }
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
+      for (int d = 4; d < 32; d <<= 1) {
+        t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+      }
+      const float m0 = fmaxf(m[n][0], t0), m1 = fmaxf(m[n][1], t1);
+      const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+      if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1])) {
+        const float c0 = exp2_fast(m[n][0] - b0), c1 = exp2_fast(m[n][1] - b1);
+        l[n][0] *= c0;
+        l[n][1] *= c1;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          uint32_t a[4];
-          load_matrices(a, (buf + k_at + t * 16 * S::kRow) ^ (i * 32));
-#pragma unroll
-          for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+          o[n][i][0] *= c0;
+          o[n][i][1] *= c1;
+          o[n][i][2] *= c0;
+          o[n][i][3] *= c1;
         }
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[t][n][j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
-      }
-      if (seen != kAll) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            if (!((seen >> (t * 16 + lane / 4)) & 1)) y[t][n][0] = y[t][n][1] = -INFINITY;
-            if (!((seen >> (t * 16 + lane / 4 + 8)) & 1)) y[t][n][2] = y[t][n][3] = -INFINITY;
-          }
-      }
-      uint32_t pb[MT][NG][2];
-#pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          t0 = fmaxf(t0, fmaxf(y[t][n][0], y[t][n][2]));
-          t1 = fmaxf(t1, fmaxf(y[t][n][1], y[t][n][3]));
-        }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
-          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
-        }
-        const float m0 = fmaxf(m[n][0], t0), m1 = fmaxf(m[n][1], t1);
-        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
-        if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1])) {
-          const float c0 = exp2_fast(m[n][0] - b0), c1 = exp2_fast(m[n][1] - b1);
-          l[n][0] *= c0;
-          l[n][1] *= c1;
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            o[n][i][0] *= c0;
-            o[n][i][1] *= c1;
-            o[n][i][2] *= c0;
-            o[n][i][3] *= c1;
-          }
-          m[n][0] = m0;
-          m[n][1] = m1;
-        }
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const float p0 = exp2_fast(y[t][n][0] - b0), p1 = exp2_fast(y[t][n][1] - b1);
-          const float p2 = exp2_fast(y[t][n][2] - b0), p3 = exp2_fast(y[t][n][3] - b1);
-          l[n][0] += p0 + p2;
-          l[n][1] += p1 + p3;
-          pb[t][n][0] = transpose8(pack2<T>(p0, p1));
-          pb[t][n][1] = transpose8(pack2<T>(p2, p3));
-        }
+        m[n][0] = m0;
+        m[n][1] = m1;
       }
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          uint32_t a[4];
-          load_matrices_t(a, (buf + S::kHalf + v_at + t * 16 * S::kRow) ^ (i * 32));
-#pragma unroll
-          for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[t][n][0], pb[t][n][1]);
-        }
-      __syncwarp();                       // every lane is done with this stage
-#pragma unroll
-      for (int i = 0; i + 1 < S::kStages - 1; ++i) mask[i] = mask[i + 1];
-      mask[S::kStages - 2] = 0;
-      const int kn = k + S::kStages - 1;
-      const int next = page_of(kn + 1);
-      if (kn < k1) mask[S::kStages - 2] = fetch(kn, st == 0 ? S::kStages - 1 : st - 1, page);
-      page = next;
-      copy_commit();
-      st = st + 1 == S::kStages ? 0 : st + 1;
+      for (int t = 0; t < MT; ++t) {
+        const float p0 = exp2_fast(y[t][n][0] - b0), p1 = exp2_fast(y[t][n][1] - b1);
+        const float p2 = exp2_fast(y[t][n][2] - b0), p3 = exp2_fast(y[t][n][3] - b1);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+        pb[t][n][0] = transpose8(pack2<T>(p0, p1));
+        pb[t][n][1] = transpose8(pack2<T>(p2, p3));
+      }
     }
-    copy_wait<0>();
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        uint32_t a[4];
+        load_matrices_t(a, (buf + S::kHalf + v_at + t * 16 * S::kRow) ^ (i * 32));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[t][n][0], pb[t][n][1]);
+      }
+    __syncwarp();                         // every lane is done with this stage
+    --ahead;
+    mask[0] = mask[1];
+    fetch();
+    advance();
+    const int used = st;
+    st = st + 1 == S::kStages ? 0 : st + 1;
+    if (--row.blocks > 0) continue;
 
-    // the four warps' sums, through shared memory (each in its own ring)
-    float* mine = reinterpret_cast<float*>(smem + warp * S::kWarpBytes);
+    // The row is done.  The four warps' sums, through the stage that each has just used;
+    // the next row's first tiles and queries are on their way meanwhile.
+    const Row done = row;
+    const bool more = ahead_row;
+    if (more) {
+      row = next;
+      ahead_row = false;
+      load_queries();
+    }
+    float* mine = reinterpret_cast<float*>(smem + warp * S::kWarpBytes + used * 2 * S::kHalf);
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
 #pragma unroll
@@ -495,10 +549,11 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
       }
     }
     __syncthreads();
-    const bool whole = k0 == 0 && k1 == nb;
-    const long long slot = 2 * static_cast<long long>(blockIdx.x) + (at == share.start ? 0 : 1);
-    for (int f = tid; f < heads * (D / 2); f += kWarps * 32) {
-      const int h = f / (D / 2), d = (f % (D / 2)) * 2;
+    const int g = done.row / p.tiles, tile = done.row - g * p.tiles;
+    const int head0 = g * p.group + tile * kHeads, heads = min(kHeads, p.group - tile * kHeads);
+    const long long slot = 2 * static_cast<long long>(blockIdx.x) + (first_row ? 0 : 1);
+    for (int f0 = tid; f0 < heads * (D / 2); f0 += kWarps * 32) {
+      const int h = f0 / (D / 2), d = (f0 % (D / 2)) * 2;
       float mx = sm_m[0][h];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][h]);
@@ -507,13 +562,14 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float c = exp2_fast(sm_m[w][h] - base);
-        const float* other = reinterpret_cast<const float*>(smem + w * S::kWarpBytes) + h * kPad + d;
+        const float* other =
+            reinterpret_cast<const float*>(smem + w * S::kWarpBytes + used * 2 * S::kHalf) + h * kPad + d;
         lt += sm_l[w][h] * c;
         a0 += other[0] * c;
         a1 += other[1] * c;
       }
-      if (whole) {
-        const long long r = static_cast<long long>(b) * p.HQ + head0 + h;
+      if (done.whole) {
+        const long long r = static_cast<long long>(done.b) * p.HQ + head0 + h;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         reinterpret_cast<uint32_t*>(p.out)[(r * D + d) / 2] = pack2<T>(a0 * inv, a1 * inv);
         if (d == 0 && p.lse) p.lse[r] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
@@ -523,46 +579,51 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
           *reinterpret_cast<float2*>(p.part_ml + (slot * kHeads + h) * 2) = make_float2(mx, lt);
       }
     }
-    __syncthreads();                      // the ring is free for the next row
-    at += k1 - k0;
-    if (row == rows - 1 && k1 == nb) {
-      before += nb;
-      ++b;
-    }
+    if (!more) break;
+    __syncthreads();                      // the stage and the warps' sums are free
+    first_row = false;
+    clear();
+    advance();
+    if (ahead < 2) fetch();
   }
 }
 
 // Adds up the parts of the rows that were cut: o = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-// CTA (c, y): values 512 y ... of the row whose last part is share c's, if one is.  128
-// threads take four values each, two groups of them every other part.
-constexpr int kJoinThreads = 256, kJoinValues = 512, kJoinParts = 3 * kSMs;
+// CTA (x, y): kValues values from y kValues of the row of cut[x].  kValues / 4 threads take
+// four values each; the CTA's groups of them take every kGroups-th part.  Few rows have many
+// parts each: then a CTA takes few values and has many groups (131072 tokens in 148 parts:
+// 56 us with 512 values and 2 groups, 51 us with 128 and 8).
+constexpr int kJoinThreads = 256, kJoinParts = 2 * kSMs;
 
-template <typename T, int D, int NG>
+template <typename T, int D, int NG, int kValues>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnArgs p) {
-  constexpr int kHeads = 8 * NG, kHere = kJoinValues / D;     // heads of a row, of this CTA
+  constexpr int kHeads = 8 * NG, kHere = kValues > D ? kValues / D : 1;   // heads of a row, of this CTA
+  constexpr int kQuads = kValues / 4, kGroups = kJoinThreads / kQuads;
   __shared__ float2 ml[kJoinParts][kHere];
-  __shared__ float4 acc[kJoinValues / 4];
-  __shared__ float sum[kJoinValues / 4];
-  const int tid = threadIdx.x, y = blockIdx.y;
+  __shared__ float4 acc[kGroups][kQuads];
+  __shared__ float sum[kGroups][kQuads];
+  const int tid = threadIdx.x, head0 = blockIdx.y * kValues / D;
   grid_wait();
   const int4 cut = p.cut[blockIdx.x];
   if (cut.x < 0) return;
-  const int g = cut.y / p.tiles, tile = cut.y % p.tiles, parts = blockIdx.x - cut.z + 1;
-  if (y * kHere >= p.group - tile * kHeads) return;           // heads past the group's
-  auto slot = [&](int i) { return 2 * static_cast<long long>(cut.z + i) + (i == 0 ? cut.w : 0); };
+  const int g = cut.y / p.tiles, tile = cut.y % p.tiles, c1 = cut.w >> 1, parts = c1 - cut.z + 1;
+  if (head0 >= p.group - tile * kHeads) return;               // heads past the group's
+  auto slot = [&](int i) { return 2 * static_cast<long long>(cut.z + i) + (i == 0 ? cut.w & 1 : 0); };
   for (int f = tid; f < parts * kHere; f += kJoinThreads)
-    ml[f / kHere][f % kHere] = reinterpret_cast<const float2*>(p.part_ml)[slot(f / kHere) * kHeads + y * kHere + f % kHere];
+    ml[f / kHere][f % kHere] =
+        reinterpret_cast<const float2*>(p.part_ml)[slot(f / kHere) * kHeads + head0 + f % kHere];
   __syncthreads();
-  const int quad = tid % (kJoinValues / 4), half = tid / (kJoinValues / 4);
-  const int hc = quad * 4 / D;
+  const int quad = tid % kQuads, group = tid / kQuads;
+  const int hc = quad * 4 / D;                                // this thread's head of kHere
   float mx = -INFINITY;
+#pragma unroll 4
   for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ml[i][hc].x);
   const float base = mx == -INFINITY ? 0.f : mx;
-  const float4* from = reinterpret_cast<const float4*>(p.part_o) + y * (kJoinValues / 4) + quad;
+  const float4* from = reinterpret_cast<const float4*>(p.part_o) + blockIdx.y * kQuads + quad;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
 #pragma unroll 8
-  for (int i = half; i < parts; i += 2) {
+  for (int i = group; i < parts; i += kGroups) {
     const float4 v = from[slot(i) * (kHeads * D / 4)];
     const float w = exp2_fast(ml[i][hc].x - base);
     l += w * ml[i][hc].y;
@@ -571,22 +632,26 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     a.z += w * v.z;
     a.w += w * v.w;
   }
-  if (half) {
-    acc[quad] = a;
-    sum[quad] = l;
-  }
+  acc[group][quad] = a;
+  sum[group][quad] = l;
   __syncthreads();
-  const int h = tile * kHeads + y * kHere + hc;
-  if (half || h >= p.group) return;
-  const float4 v = acc[quad];
-  l += sum[quad];
+  const int h = tile * kHeads + head0 + hc;
+  if (group || h >= p.group) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) {
+    const float4 v = acc[i][quad];
+    l += sum[i][quad];
+    a.x += v.x;
+    a.y += v.y;
+    a.z += v.z;
+    a.w += v.w;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const long long r = static_cast<long long>(cut.x) * p.HQ + g * p.group + h;
-  reinterpret_cast<uint2*>(p.out)[(r * D + quad * 4 % D) / 4] =
-      make_uint2(pack2<T>((a.x + v.x) * inv, (a.y + v.y) * inv),
-                 pack2<T>((a.z + v.z) * inv, (a.w + v.w) * inv));
-  if (quad * 4 % D == 0 && p.lse)
-    p.lse[r] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+  const int d = (blockIdx.y * kValues + quad * 4) % D;
+  reinterpret_cast<uint2*>(p.out)[(r * D + d) / 4] =
+      make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
+  if (d == 0 && p.lse) p.lse[r] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
@@ -598,33 +663,54 @@ int heads_of(int group) { return group <= 8 ? 8 : 16; }
 int block_of(int D) { return D == 64 ? Shape<64>::kBlock : D == 128 ? Shape<128>::kBlock : Shape<256>::kBlock; }
 int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
 
-// CTAs of a call: what the GPU holds at once, or one per block of tokens if there are fewer
-long long grid_of(int B, int HQ, int HKV, int D, long long max_tokens) {
+// Rows of up to 4 blocks are not cut, and of up to 8 where there is a row for every CTA: one
+// CTA takes such a row in less than the cut's partial sums and the join cost.  Not cut / cut:
+// 1 row of 100 tokens of 128 dims 5.8 / 7.1 us, of 512 tokens 10.7 / 7.1 us; 512 rows of
+// 256 tokens 14.8 / 22.1 us, of 500 tokens 22.4 / 30.5 us.
+constexpr int kWhole = 4, kWholeMany = 8;
+
+struct Plan {
+  long long rows, grid;      // rows of a call; CTAs: what the GPU holds at once, or fewer
+  bool split;                // whether rows may be cut
+  size_t cut, bytes;         // entries of `cut`, workspace
+};
+
+Plan plan_of(int B, int HQ, int HKV, int D, long long max_tokens) {
+  Plan q;
   const int heads = heads_of(HQ / HKV);
-  const long long rows = static_cast<long long>(B) * HKV * ((HQ / HKV + heads - 1) / heads);
+  q.rows = static_cast<long long>(B) * HKV * ((HQ / HKV + heads - 1) / heads);
   const long long nb = max_tokens > 0 ? (max_tokens + block_of(D) - 1) / block_of(D) : 1;
   const long long most = static_cast<long long>(kSMs) * resident(D);
-  return rows * nb < most ? rows * nb : most;
+  q.split = nb > (q.rows >= most ? kWholeMany : kWhole);
+  const long long units = q.rows * (q.split ? nb : 1);
+  q.grid = units < most ? units : most;
+  q.cut = static_cast<size_t>(q.rows <= q.grid ? q.rows : q.grid);
+  q.bytes = q.split ? q.cut * sizeof(int4) + static_cast<size_t>(q.grid) * 2 * heads * (D + 2) * 4 : 0;
+  return q;
 }
 
 template <typename T, int D, int NG>
-cudaError_t launch_shape(const AttnArgs& p, cudaStream_t st) {
+cudaError_t launch_shape(const AttnArgs& p, const Plan& q, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<T, D, NG>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   attn_decode_kernel<T, D, NG><<<p.grid, kWarps * 32, Shape<D>::kSmem, st>>>(p);
   e = cudaGetLastError();
-  if (e != cudaSuccess || !p.cut) return e;
-  return launch_after(attn_join_kernel<T, D, NG>, dim3(p.grid, 8 * NG * D / kJoinValues),
-                      dim3(kJoinThreads), 0, st, p);
+  if (e != cudaSuccess || !q.split) return e;
+  const unsigned x = static_cast<unsigned>(q.cut);
+  if (q.rows * 8 <= q.grid)
+    return launch_after(attn_join_kernel<T, D, NG, 128>, dim3(x, 8 * NG * D / 128), dim3(kJoinThreads),
+                        0, st, p);
+  return launch_after(attn_join_kernel<T, D, NG, 512>, dim3(x, 8 * NG * D / 512), dim3(kJoinThreads), 0,
+                      st, p);
 }
 
 template <typename T>
-cudaError_t launch(const AttnArgs& p, int D, cudaStream_t st) {
+cudaError_t launch(const AttnArgs& p, int D, const Plan& q, cudaStream_t st) {
   const bool wide = p.group > 8;
-  if (D == 64) return wide ? launch_shape<T, 64, 2>(p, st) : launch_shape<T, 64, 1>(p, st);
-  if (D == 128) return wide ? launch_shape<T, 128, 2>(p, st) : launch_shape<T, 128, 1>(p, st);
-  return wide ? launch_shape<T, 256, 2>(p, st) : launch_shape<T, 256, 1>(p, st);
+  if (D == 64) return wide ? launch_shape<T, 64, 2>(p, q, st) : launch_shape<T, 64, 1>(p, q, st);
+  if (D == 128) return wide ? launch_shape<T, 128, 2>(p, q, st) : launch_shape<T, 128, 1>(p, q, st);
+  return wide ? launch_shape<T, 256, 2>(p, q, st) : launch_shape<T, 256, 1>(p, q, st);
 }
 
 }  // namespace
@@ -633,9 +719,7 @@ extern "C" {
 
 size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D, int max_tokens) {
   if (B < 1 || HQ < 1 || HKV < 1 || HQ % HKV != 0 || (D != 64 && D != 128 && D != 256)) return 0;
-  if (max_tokens <= block_of(D)) return 0;    // no row is ever cut
-  return static_cast<size_t>(grid_of(B, HQ, HKV, D, max_tokens)) *
-         (2 * static_cast<size_t>(heads_of(HQ / HKV)) * (D + 2) * 4 + sizeof(int4));
+  return plan_of(B, HQ, HKV, D, max_tokens).bytes;
 }
 
 int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
@@ -667,11 +751,13 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] % 8 || v_strides[i] % 8)
       return GDN_ERR_ALIGN;
-  const int max_tokens = table_width * page_size;
-  const size_t need = gdn_paged_attention_workspace_bytes(B, HQ, HKV, D, max_tokens);
-  if (need > 0 && !workspace) return GDN_ERR_NULL;
+  // no row sees more than its table holds, or its window and sinks
+  const int held = table_width * page_size;
+  const int max_tokens = window > 0 && window + num_sinks < held ? window + num_sinks : held;
+  const Plan plan = plan_of(B, HQ, HKV, D, max_tokens);
+  if (plan.bytes > 0 && !workspace) return GDN_ERR_NULL;
   if (!aligned(workspace, 16)) return GDN_ERR_ALIGN;
-  if (workspace_bytes < need) return GDN_ERR_SHAPE;
+  if (workspace_bytes < plan.bytes) return GDN_ERR_SHAPE;
   AttnArgs p{};
   p.q = q; p.k = static_cast<char*>(k_cache); p.v = static_cast<char*>(v_cache);
   p.tables = block_tables; p.lens = seq_lens; p.k_new = k_new; p.v_new = v_new;
@@ -685,16 +771,17 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   p.page_size = page_size; p.width = table_width; p.window = window;
   p.sinks = window > 0 ? num_sinks : 0;
   p.tiles = (p.group + heads_of(p.group) - 1) / heads_of(p.group);
-  p.grid = static_cast<int>(grid_of(B, HQ, HKV, D, max_tokens));
-  if (need > 0) {
+  p.grid = static_cast<int>(plan.grid);
+  if (plan.split) {
     p.cut = static_cast<int4*>(workspace);
-    p.part_o = reinterpret_cast<float*>(p.cut + p.grid);
+    p.part_o = reinterpret_cast<float*>(p.cut + plan.cut);
     p.part_ml = p.part_o + static_cast<size_t>(2 * p.grid) * heads_of(p.group) * D;
+    p.by_row = plan.rows <= plan.grid;
   }
   p.twin = p.k_page == p.v_page && p.k_tok == p.v_tok;
   div_constants(static_cast<uint32_t>(page_size), p.page_mul, p.page_shift);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, st) : launch<__half>(p, D, st);
+  const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, plan, st) : launch<__half>(p, D, plan, st);
   return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
 

@@ -159,8 +159,8 @@ def paged_attention_decode(
         _need(output, "output", dt, (B, 1, HQ, D), dev)
     _check_counter(bad_index_count, dev)
     lse = q.new_empty((B, HQ), dtype=_F32)
-    nbytes = _workspace_bytes("gdn_paged_attention_workspace_bytes", B, HQ, HKV, D,
-                              width * page_size)
+    most = min(width * page_size, window + num_sinks) if window else width * page_size
+    nbytes = _workspace_bytes("gdn_paged_attention_workspace_bytes", B, HQ, HKV, D, most)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(
         dev, "gdn_paged_attention_decode", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
