@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 // more of them than the list holds (many equal scores) the ranks come from binary searches
 // in the sorted lists instead.
 
-constexpr int kMergeList = 1024;
+constexpr int kMergeList = 1024, kHeld = 8;
 
 struct MergeItem {
   unsigned long long score;      // of the 64-bit score, in an order-preserving form
@@ -472,10 +472,16 @@ __device__ __forceinline__ double ln_sum(double t) {
 }
 
 // sum over a group of 8 lanes; groups of one warp may have left the loop
-__device__ __forceinline__ int sum8(int x) {
+template <typename T> __device__ __forceinline__ T sum8(T x) {
   const uint32_t mask = 0xffu << (threadIdx.x & 24);
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
+  return x;
+}
+__device__ __forceinline__ float max8(float x) {
+  const uint32_t mask = 0xffu << (threadIdx.x & 24);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(mask, x, o));
   return x;
 }
 
@@ -485,7 +491,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   __shared__ MergeItem item[kMergeList];
   __shared__ int count, alive;
   __shared__ bool done[kMaxBeams];
-  const int b = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int b = blockIdx.x, tid = threadIdx.x;
   const int per_beam = p.slices * p.n, lists = p.K * p.slices, total = lists * p.n;
   if (tid == 0) {
     count = alive = 0;
@@ -498,38 +504,48 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   }
   __syncthreads();
   grid_wait();
-  for (int i = warp; i < p.K; i += kMergeThreads / 32) {
+  // everything that is read comes at once: up to kHeld keys a thread, the first candidates
+  // (the first `depth` of every slice, of as many slices as fit; at least n where there are
+  // as many), and the slices' sums, eight threads to a beam
+  const unsigned long long* all = p.keys + static_cast<long long>(b) * total;
+  unsigned long long held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int f = u * kMergeThreads + tid;
+    held[u] = f < total ? all[f] : 0;
+  }
+  const int depth = (p.n + lists - 1) / lists, items = min(lists * depth, kHeadItems);
+  const unsigned long long head_key = tid < items ? all[tid % lists * p.n + tid / lists] : 0;
+  const int i8 = tid / 8;
+  if (i8 < p.K) {
     double l = NAN;                     // not finite: a beam without candidates of its own
-    if (!done[i] && isfinite(cum[i])) {
-      const float2* sums = p.sums + (static_cast<long long>(b) * p.K + i) * p.slices;
-      float m = -INFINITY;
-      for (int s = lane; s < p.slices; s += 32) m = fmaxf(m, sums[s].x);
-      m = warp_max(m);
-      double t = 0.0;
-      for (int s = lane; s < p.slices; s += 32) {
+    const bool on = !done[i8] && isfinite(cum[i8]);
+    const float2* sums = p.sums + (static_cast<long long>(b) * p.K + i8) * p.slices;
+    float m = -INFINITY;
+    if (on)
+      for (int s = tid % 8; s < p.slices; s += 8) m = fmaxf(m, sums[s].x);
+    m = max8(m);
+    double t = 0.0;
+    if (on)
+      for (int s = tid % 8; s < p.slices; s += 8) {
         const float2 ms = sums[s];
         if (ms.x > -INFINITY || isnan(ms.y))
           t += static_cast<double>(ms.y) * static_cast<double>(exp2f((ms.x - m) * kLog2e));
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (isfinite(m) && t >= 0.5 && t < 1e300) l = m + ln_sum(t);
-    }
-    if (lane == 0) lse[i] = l;
+    t = sum8(t);
+    if (on && isfinite(m) && t >= 0.5 && t < 1e300) l = m + ln_sum(t);
+    if (tid % 8 == 0) lse[i8] = l;
   }
   __syncthreads();
-  const unsigned long long* all = p.keys + static_cast<long long>(b) * total;
   auto score_of = [&](int i, unsigned long long k) {
     return cum[i] + (static_cast<double>(key_logit(k)) - lse[i]);
   };
-  // the first `depth` candidates of every slice (of as many slices as fit), at least n where
-  // there are as many
-  const int depth = (p.n + lists - 1) / lists, items = min(lists * depth, kHeadItems);
+  // a slice that wrote nothing (its beam is finished or dead) leaves stale keys: lse says so
   if (tid < items) {
-    const int list = tid % lists, i = list / p.slices;
-    const unsigned long long k = isfinite(lse[i]) ? all[list * p.n + tid / lists] : 0;
-    head[tid] = ordered(k ? score_of(i, k) : -INFINITY);
+    const int i = tid % lists / p.slices;
+    head[tid] = ordered(head_key && isfinite(lse[i]) ? score_of(i, head_key) : -INFINITY);
   }
+  __syncthreads();
   __syncthreads();
   // eight threads count for one
   for (int f = tid / 8; f < items; f += kMergeThreads / 8) {
@@ -542,24 +558,19 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   __syncthreads();
   const double low = bound;
   int valid = 0;
-  for (int f0 = 0; f0 < total; f0 += 4 * kMergeThreads) {
-    unsigned long long k[4];
+  auto take = [&](int f, unsigned long long k) {
+    const int i = f / per_beam;
+    if (k == 0 || !isfinite(lse[i])) return;
+    ++valid;
+    const double sc = score_of(i, k);
+    if (!(sc >= low)) return;
+    const int at = next_place(&count);
+    if (at < kMergeList) item[at] = MergeItem{ordered(sc), k, i};
+  };
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int f = f0 + u * kMergeThreads + tid;
-      k[u] = f < total && isfinite(lse[f / per_beam]) ? all[f] : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = (f0 + u * kMergeThreads + tid) / per_beam;
-      if (k[u] == 0) continue;
-      ++valid;
-      const double sc = score_of(i, k[u]);
-      if (!(sc >= low)) continue;
-      const int at = atomicAdd(&count, 1);
-      if (at < kMergeList) item[at] = MergeItem{ordered(sc), k[u], i};
-    }
-  }
+  for (int u = 0; u < kHeld; ++u)
+    if (u * kMergeThreads + tid < total) take(u * kMergeThreads + tid, held[u]);
+  for (int f = kHeld * kMergeThreads + tid; f < total; f += kMergeThreads) take(f, all[f]);
   if (tid < p.K && done[tid] && isfinite(cum[tid])) {
     ++valid;
     if (cum[tid] >= low) {

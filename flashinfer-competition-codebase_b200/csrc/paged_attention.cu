@@ -691,8 +691,7 @@ Plan plan_of(int B, int HQ, int HKV, int D, long long max_tokens) {
 
 template <typename T, int D, int NG>
 cudaError_t launch_shape(const AttnArgs& p, const Plan& q, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<T, D, NG>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  cudaError_t e = allow_smem<attn_decode_kernel<T, D, NG>>(Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
   attn_decode_kernel<T, D, NG><<<p.grid, kWarps * 32, Shape<D>::kSmem, st>>>(p);
   e = cudaGetLastError();

@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gdn_b200.h"
 
 namespace gdn_serving {
@@ -63,6 +65,19 @@ cudaError_t launch_after(void (*kernel)(Args...), dim3 grid, dim3 block, size_t 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device: the attribute call
+// costs the host microseconds, a decode step's call not many more.
+template <auto kKernel> cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};       // one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
