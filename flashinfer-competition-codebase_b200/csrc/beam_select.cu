@@ -109,7 +109,7 @@ struct SliceShared {
   int at[kList];                   // their places in the row
   unsigned long long list[kList];  // keys of candidates
   float red[kWarps];
-  double sum[kWarps];
+  float sum[kWarps];
   int scan[kWarps];
   unsigned long long best[kWarps];
   float sample[kThreads];        // of the keys, where they overflow
@@ -159,18 +159,23 @@ __device__ __forceinline__ int next_place(int* count) {
   return at;
 }
 
-// Descending bitonic sort of one value per lane.
-__device__ __forceinline__ float sort_lanes(float x, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int step = size / 2; step > 0; step >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, x, step);
-      const bool up = (lane & size) != 0;            // this run ascends (the last never does)
-      const bool low = (lane & step) == 0;
-      x = (low != up) ? fmaxf(x, y) : fminf(x, y);
-    }
-  return x;
+// The warp's largest x, by one reduction; NaNs do not count.
+__device__ __forceinline__ float warp_largest(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The warp's r-th largest x, equal ones counted one by one.
+__device__ __forceinline__ float warp_nth(float x, int r) {
+  float y = warp_largest(x);
+  for (int i = 1; i < r; ++i) {
+    const uint32_t same = __ballot_sync(0xffffffffu, x == y);
+    if (same == 0u) return -INFINITY;                  // only NaNs are left
+    if (threadIdx.x % 32 == __ffs(same) - 1) x = -INFINITY;
+    y = warp_largest(x);
+  }
+  return y;
 }
 
 // Writes the largest n of c <= kList keys, descending, 0 where there are fewer.
@@ -178,6 +183,7 @@ __device__ void write_ranked(const unsigned long long* list, int c, int n, unsig
   for (int i = threadIdx.x; i < c; i += kThreads) {
     const unsigned long long k = list[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < c; ++j) rank += list[j] > k;
     if (rank < n) out[rank] = k;
   }
@@ -193,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   grid_trigger();                // the merge may take its place once the last slices run
   // a finished or dead beam's logits decide nothing
-  if ((p.finished && p.finished[row]) || !isfinite(p.scores[row])) return;
+  const bool done = p.finished != nullptr && p.finished[row];
+  if (done | !isfinite(p.scores[row])) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + b * p.stride_batch + i * p.stride_beam;
   // the row as aligned 16-byte vectors; vector c holds tokens c E - mis ...; the first and the
   // last may be partial and are handled one by one
@@ -230,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) m = fmaxf(m, v[k].largest());
   {
-    const float sorted = sort_lanes(m, lane);
-    if (lane == (p.n + kWarps - 1) / kWarps - 1) sh.red[warp] = sorted;
+    const float nth = warp_nth(m, (p.n + kWarps - 1) / kWarps);
+    if (lane == 0) sh.red[warp] = nth;
   }
   __syncthreads();
   float bound = sh.red[0];
@@ -294,31 +301,29 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     for (int k = 0; k < kBatch; ++k) v[k] = next[k];
   }
   // the CTA's maximum and sum
-  const float wm = warp_max(m);
+  const float wm = warp_largest(m);
   if (lane == 0) sh.red[warp] = wm;
   __syncthreads();
   m = sh.red[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.red[w]);
   const float held = fminf(fmaxf(m, -kHuge), kHuge), c1 = held * kLog2e;
-  double s = static_cast<double>(sums.total()) *
-             static_cast<double>(exp2_fast(c0 - c1));
+  float part = sums.total() * exp2_fast(c0 - c1);
   const int e0 = max(0, v0 * E - mis), e1 = min(p.V, v1 * E - mis);   // the slice's tokens
   if (held != m && isfinite(m)) {
-    s = 0.0;
+    part = 0.f;
     for (int t = e0 + tid; t < e1; t += kThreads) {
       const float y = to_f(x[t]);
-      s += isnan(y) ? NAN : y == m ? 1.0 : 0.0;
+      part += isnan(y) ? NAN : y == m ? 1.f : 0.f;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) sh.sum[warp] = s;
+  part = warp_sum(part);
+  if (lane == 0) sh.sum[warp] = part;
   __syncthreads();
   if (tid == 0) {
-    s = sh.sum[0];
+    double s = 0.0;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) s += sh.sum[w];
+    for (int w = 0; w < kWarps; ++w) s += static_cast<double>(sh.sum[w]);
     if (held == m) s *= static_cast<double>(exp2f(-fmaf(held, kLog2e, -c1)));   // what c's rounding took
     p.sums[static_cast<long long>(row) * p.slices + slice] = make_float2(m, static_cast<float>(s));
   }
@@ -326,8 +331,8 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   const int aside = min(sh.count, kList), wide = min(aside, kThreads) / 32;
   const int nth = wide > 0 ? (p.n + wide - 1) / wide : 33;
   if (warp < wide && nth <= 32) {
-    const float sorted = sort_lanes(V{sh.vec[tid]}.largest(), lane);
-    if (lane == nth - 1) sh.red[warp] = sorted;
+    const float y = warp_nth(V{sh.vec[tid]}.largest(), nth);
+    if (lane == 0) sh.red[warp] = y;
   }
   __syncthreads();
   if (nth <= 32) {               // at least the bound before
