@@ -22,6 +22,7 @@ using namespace gdn_serving;
 
 constexpr int kMaxPools = 32;
 constexpr int kMaxPairs = 4096;
+constexpr int kMaxPages = 1 << 30;
 constexpr int kThreads = 256;
 constexpr int kVecs = 16;          // 16-byte vectors a thread holds: 64 KB per CTA
 
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
 
 int check_pools(void* const* pools, const int64_t* bytes, const int64_t* pitch, int num_pools,
                 int num_pages, Pools& out, int& unit) {
-  if (num_pools < 0 || num_pages < 1) return GDN_ERR_SHAPE;
+  if (num_pools < 0 || num_pages < 1 || num_pages > kMaxPages) return GDN_ERR_SHAPE;
   if (num_pools > kMaxPools) return GDN_ERR_LIMIT;
   if (num_pools > 0 && (!pools || !bytes || !pitch)) return GDN_ERR_NULL;
   memset(&out, 0, sizeof(out));
@@ -585,7 +586,7 @@ int gdn_copy_pages(void* const* pools, const int64_t* page_bytes, const int64_t*
 
 int gdn_alloc_pages(int32_t* refcounts, int num_pages, const uint8_t* need, int n, int32_t* pages,
                     void* workspace, size_t workspace_bytes, void* stream) {
-  if (num_pages < 1 || n < 0) return GDN_ERR_SHAPE;
+  if (num_pages < 1 || num_pages > kMaxPages || n < 0) return GDN_ERR_SHAPE;
   if (n == 0) return GDN_OK;
   if (!refcounts || !need || !pages || !workspace) return GDN_ERR_NULL;
   if (!aligned(refcounts, 4) || !aligned(pages, 4) || !aligned(workspace, 4)) return GDN_ERR_ALIGN;
@@ -597,7 +598,7 @@ int gdn_alloc_pages(int32_t* refcounts, int num_pages, const uint8_t* need, int 
 
 int gdn_free_pages(int32_t* refcounts, int num_pages, const int32_t* pages, int64_t n,
                    int32_t* bad_index_count, void* stream) {
-  if (num_pages < 1 || n < 0) return GDN_ERR_SHAPE;
+  if (num_pages < 1 || num_pages > kMaxPages || n < 0) return GDN_ERR_SHAPE;
   if (n == 0) return GDN_OK;
   if (!refcounts || !pages) return GDN_ERR_NULL;
   if (!aligned(refcounts, 4) || !aligned(pages, 4) || !aligned(bad_index_count, 4))

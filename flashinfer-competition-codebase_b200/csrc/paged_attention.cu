@@ -733,7 +733,8 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   if (D != 64 && D != 128 && D != 256) return GDN_ERR_SHAPE;
   if (B < 0 || HQ < 1 || HKV < 1 || HQ % HKV != 0) return GDN_ERR_SHAPE;
   if (num_pages < 1 || page_size < 1 || table_width < 0) return GDN_ERR_SHAPE;
-  if (static_cast<long long>(table_width) * page_size > 0x7fffffffLL - 1024) return GDN_ERR_SHAPE;
+  if (static_cast<long long>(table_width) * page_size > 0x7fffffffLL - 1024 || table_stride < 0)
+    return GDN_ERR_SHAPE;
   if (B > 65535 || static_cast<long long>(B) * HQ > 0x7fffffffLL / 256) return GDN_ERR_SHAPE;
   if (dtype != GDN_DTYPE_BF16 && dtype != GDN_DTYPE_FP16) return GDN_ERR_ARG;
   if (window < 0 || num_sinks < 0 || window > 0x3fffffff || num_sinks > 0x3fffffff) return GDN_ERR_ARG;
@@ -750,6 +751,14 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] % 8 || v_strides[i] % 8)
       return GDN_ERR_ALIGN;
+  const size_t out_bytes = static_cast<size_t>(B) * HQ * D * 2;
+  auto cache_bytes = [&](const int64_t* st) {
+    return 2 * static_cast<size_t>((num_pages - 1) * st[0] + (page_size - 1) * st[1] + (HKV - 1) * st[2] + D);
+  };
+  if (overlaps(output, out_bytes, q, out_bytes) ||
+      overlaps(output, out_bytes, k_cache, cache_bytes(k_strides)) ||
+      overlaps(output, out_bytes, v_cache, cache_bytes(v_strides)) || (k_new && k_cache == v_cache))
+    return GDN_ERR_ALIAS;
   // no row sees more than its table holds, or its window and sinks
   const int held = table_width * page_size;
   const int max_tokens = window > 0 && window + num_sinks < held ? window + num_sinks : held;

@@ -2,13 +2,12 @@
 
 Tolerance.  A score is cum + (x - lse) in 64 bits, rounded once to fp32 (2^-24 relative).
 lse's error is the softmax-weighted mean of its terms' relative errors.  A term's exponent
-(x - m) log2 e is rounded in the subtraction, in the factor and in the product: at most
-3 |x - m| 2^-24 in the exponent to e, whose weighted mean is at most 3 ln V 2^-24 < 40 2^-24;
-the exponential is off by 2^-22; a chain of k positive fp32 additions by k 2^-24, here k at most
-17 x 4 / 4 + 2 for fp32 and 9 x 8 / 4 + 2 for 16-bit logits (a thread's vectors in four chains), 64 bits
-beyond, and 2^-24 for a slice's sum.  Together below (40 + 4 + 20 + 1) 2^-24 < 4e-6.  Two
-candidates of different beams whose scores are nearer than twice that may come in either
-order; all others must come exactly.
+x log2 e - c is rounded once and its factor once: at most 1.5 |x - m| 2^-24 in the exponent to
+e, whose weighted mean is at most 1.5 ln V 2^-24 < 20 2^-24; the exponential is off by 2^-22; a
+chain of k positive fp32 additions by k 2^-24, here k <= 40 (a thread's at most 16 vectors in
+four chains, then the warp's lanes), 64 bits beyond, and 2^-24 for a slice's sum.  Together
+(20 + 4 + 40 + 1) 2^-24 < 4e-6.  Two candidates of different beams whose scores are nearer
+than twice that may come in either order; all others must come exactly.
 """
 
 import math
@@ -79,7 +78,8 @@ def test_ties_go_to_the_lower_beam_and_token():
     assert t[0].tolist() == list(range(60))
 
 
-@pytest.mark.parametrize("order", ["ascending", "descending", "blocks"])
+@pytest.mark.parametrize("order", ["ascending", "descending", "blocks", "hot", "hot ties",
+                                   "hot and one above"])
 def test_sorted_logits(order):
     V = 60000
     row = torch.linspace(-20, 20, V)
@@ -88,8 +88,35 @@ def test_sorted_logits(order):
     if order == "blocks":                            # the best ones all side by side
         row = torch.cat([torch.full((30000,), -5.0), torch.linspace(5, 6, 64),
                          torch.full((V - 30064,), -4.0)])
+    if order.startswith("hot"):                      # large ones where a sample may miss them
+        row = torch.full((V,), -5.0)
+        row[3000:33000] = 5.0 if "ties" in order else torch.linspace(5, 6, 30000)
+        if "above" in order:
+            row[3000:33000] = 5.0
+            row[20000:20100] = 7.0
     x = row.repeat(2, 2, 1).to(torch.float32).cuda()
     check(x, torch.tensor([[-1.0, -1.5], [0.0, -30.0]]).cuda(), 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n", [1, 16, 17, 64])
+def test_hot_regions_of_every_type(dtype, n):
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(1, 2, 150001, generator=g)
+    x[0, 0, 9000:40000] += 8.0
+    x[0, 1, -3000:] += 6.0
+    check(x.to(dtype).cuda(), torch.tensor([[-1.0, -0.5]]).cuda(), n)
+
+
+def test_tokens_masked_with_the_lowest_value():
+    """A grammar's mask: a few tokens left, all others at the type's lowest value."""
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x, s = make(3, 4, 50000, dtype, seed=8)
+        keep = torch.zeros(50000, dtype=torch.bool)
+        keep[torch.tensor([5, 17, 49999, 30000, 30001])] = True
+        x[:, :, ~keep] = torch.finfo(dtype).min
+        check(x, s, 4)
+        check(x, s, 32)                              # some masked ones have to be taken
 
 
 def test_coarse_bf16_logits_with_many_ties():

@@ -97,11 +97,25 @@ def test_window_and_sinks(window, sinks):
     check(x, run(x, window=window, num_sinks=sinks), want)
 
 
-@pytest.mark.parametrize("lens", [[5000], [4097, 1, 4096], [700] * 40, [1] * 300])
+@pytest.mark.parametrize("lens", [[5000], [4097, 1, 4096], [700] * 40, [1] * 300,
+                                  [520] * 150 + [0, 1, 63, 64, 65, 2000],     # cut rows by share
+                                  [500] * 300, [64] * 200 + [3000],
+                                  [0] * 140 + [900, 0, 40]])
 def test_long_split_and_many_rows(lens):
     x = make(lens, 8, 2, 128, 16, seed=len(lens))
     want = expect(x)
     check(x, run(x), want)
+
+
+@pytest.mark.parametrize("D,HQ,HKV", [(64, 24, 1), (256, 12, 1), (256, 8, 2), (64, 4, 4), (128, 40, 1)])
+@pytest.mark.parametrize("lens", [[3001, 64, 0, 1025], [130] * 9 + [2500]])
+def test_cut_rows_of_other_shapes(D, HQ, HKV, lens):
+    x = make(lens, HQ, HKV, D, 16, seed=HQ)
+    want = expect(x)
+    check(x, run(x), want)
+    x = make(lens, HQ, HKV, D, 8, FP16, seed=HQ + 1)
+    want = expect(x, 1500, 9)
+    check(x, run(x, window=1500, num_sinks=9), want)
 
 
 def test_without_new_rows_reads_the_cache_only():

@@ -34,7 +34,12 @@ def attend(gdn_lib, **over):
     (dict(k=None), _lib.GDN_ERR_NULL), (dict(out=None), _lib.GDN_ERR_NULL),
     (dict(ks=None), _lib.GDN_ERR_NULL), (dict(q=P + 8), _lib.GDN_ERR_ALIGN),
     (dict(v=P + 2), _lib.GDN_ERR_ALIGN), (dict(lens=P + 2), _lib.GDN_ERR_ALIGN),
-    (dict(ks=L3(4096, 260, 128)), _lib.GDN_ERR_ALIGN),
+    (dict(ks=L3(4096, 260, 128)), _lib.GDN_ERR_ALIGN), (dict(stride=-1), _lib.GDN_ERR_SHAPE),
+    (dict(), _lib.GDN_ERR_ALIAS),          # keys and values stored into the same cache
+    (dict(out=P), _lib.GDN_ERR_ALIAS), (dict(out=P + 4096), _lib.GDN_ERR_ALIAS),
+    (dict(width=40, ws=None, vc=4 * P), _lib.GDN_ERR_NULL),
+    (dict(width=40, ws=P + 8, vc=4 * P), _lib.GDN_ERR_ALIGN),
+    (dict(width=40, ws_bytes=64, vc=4 * P), _lib.GDN_ERR_SHAPE),
 ])
 def test_attention_c_entry_refuses(gdn_lib, over, code):
     assert attend(gdn_lib, **over) == code
@@ -42,6 +47,16 @@ def test_attention_c_entry_refuses(gdn_lib, over, code):
 
 def test_attention_c_entry_does_nothing_for_an_empty_batch(gdn_lib):
     assert attend(gdn_lib, B=0, q=None, out=None) == _lib.GDN_OK
+
+
+def test_attention_workspace_covers_what_the_call_asks_for(gdn_lib):
+    """A windowed call needs the workspace of its window; every size of the table is enough."""
+    ws = gdn_lib.gdn_paged_attention_workspace_bytes
+    assert ws(1, 8, 2, 128, 64) == 0 and ws(0, 8, 2, 128, 4096) == 0 and ws(1, 7, 2, 128, 4096) == 0
+    for D in (64, 128, 256):
+        for B, HQ, HKV in ((1, 8, 2), (3, 48, 2), (500, 8, 8)):
+            sizes = [ws(B, HQ, HKV, D, n) for n in (1, 100, 600, 1000, 5000, 100000)]
+            assert all(a <= b for a, b in zip(sizes[-3:], sizes[-2:])) and sizes[-1] > 0
 
 
 def select(gdn_lib, **over):
@@ -74,6 +89,7 @@ def test_page_c_entries_refuse(gdn_lib):
     one = pools((P, 64, 64))
     f = gdn_lib.gdn_copy_pages
     assert f(*one, 0, P, P, 1, None, None) == _lib.GDN_ERR_SHAPE
+    assert f(*one, 2**30 + 1, P, P, 1, None, None) == _lib.GDN_ERR_SHAPE
     assert f(*one, 4, P, P, -1, None, None) == _lib.GDN_ERR_SHAPE
     assert f(*one, 4, P, P, 4097, None, None) == _lib.GDN_ERR_LIMIT
     assert f(*pools(*[(P + (i << 30), 64, 64) for i in range(33)]), 4, P, P, 1, None, None) == _lib.GDN_ERR_LIMIT
