@@ -162,6 +162,24 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         return lib
 
 
+def torch_calls():
+    """The serving operators' calls as a CPython extension (``csrc/torch_entry.cpp``), or None
+    where it is not built for this torch and Python: the same calls then go through ctypes."""
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_file_location
+
+    from .build import torch_lib_path
+
+    path = torch_lib_path()
+    if not os.path.exists(path):
+        return None
+    load()
+    loader = ExtensionFileLoader("gdn_b200_torch", path)
+    module = module_from_spec(spec_from_file_location("gdn_b200_torch", path, loader=loader))
+    loader.exec_module(module)
+    return module
+
+
 def strerror(code: int) -> str:
     return load().gdn_strerror(code).decode()
 

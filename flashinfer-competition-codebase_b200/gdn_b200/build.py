@@ -29,6 +29,8 @@ TVM_LIB_PATH = os.path.join(LIB_DIR, "libgdn_b200_tvm.so")
 # the decode library
 PROBE_LIB_PATH = os.path.join(LIB_DIR, "libgdn_b200_probe.so")
 PROBE_SOURCES = ["roofline_probe.cu"]
+# the serving operators' Python calls, for the torch and Python it is built with
+TORCH_SOURCE = "torch_entry.cpp"
 TVM_SOURCES = ["tvm_ffi_entry.cu", "gdn_decode.cu", "gdn_prefill_chunked.cu", "gdn_prefill_wy.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -143,8 +145,50 @@ def build_probe(force: bool = False) -> str:
     return PROBE_LIB_PATH
 
 
+def torch_lib_path() -> str:
+    import sysconfig
+
+    import torch
+
+    tag = f"{torch.__version__}-{sysconfig.get_config_var('SOABI')}".replace("/", "_")
+    return os.path.join(LIB_DIR, f"gdn_b200_torch-{tag}.so")
+
+
+def build_torch(force: bool = False) -> str:
+    """Compile the serving operators' Python calls (``csrc/torch_entry.cpp``), a CPython
+    extension on libgdn_b200.so and the installed torch, if missing or stale."""
+    import sysconfig
+
+    import torch
+
+    path, src = torch_lib_path(), os.path.join(SRC_DIR, TORCH_SOURCE)
+    deps = [src, os.path.join(INCLUDE_DIR, "gdn_b200.h"), os.path.abspath(__file__)]
+    if not force and os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path)
+                                                  for d in deps):
+        return path
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = path + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in (INCLUDE_DIR, os.path.join(root, "include"),
+                os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_path("include"), os.path.join(cuda, "include")):
+        cmd += ["-I", inc]
+    cmd += ["-o", tmp, src, f"-L{LIB_DIR}", "-lgdn_b200", f"-L{os.path.join(root, 'lib')}", "-lc10",
+            "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(
+            "g++ failed (%d):\n%s\n%s" % (proc.returncode, " ".join(cmd), proc.stderr[-8000:])
+        )
+    os.replace(tmp, path)
+    return path
+
+
 if __name__ == "__main__":
     force = "--force" in sys.argv
     print(build(force=force, verbose="-v" in sys.argv))
     print(build_tvm_ffi(force=force))
+    print(build_torch(force=force))
     print(build_probe(force=force))

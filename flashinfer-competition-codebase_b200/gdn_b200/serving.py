@@ -11,7 +11,10 @@ and its state pool; the reference has no counterpart:
 
 Like the entry points in ``ops.py``, each checks its tensors on the host and makes one call
 into libgdn_b200.so on their device's current stream: no host synchronisation, no CPU
-fallback.  Workspaces come from torch's caching allocator for each call, so calls on
+fallback.  The small calls are bound by that host work, so each first tries its twin in
+``csrc/torch_entry.cpp``, which makes the same checks and the same library call from C++ and
+declines whatever does not pass; what it declines is checked here, and refused in words or
+called through ctypes.  Workspaces come from torch's caching allocator for each call, so calls on
 different streams, and graphs captured from them, never share one.
 """
 
@@ -33,9 +36,33 @@ _DTYPE_CODES = {_BF16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, _F32: _l
 Pools = Union[torch.Tensor, Sequence[torch.Tensor]]
 
 
-# The small calls are bound by host work (a launch takes about 3 us), so the common case of
-# each check is one chain of comparisons, and the stream and device come from torch's
-# cheapest accessors (72 ns against 2.2 us for torch.cuda.current_stream).
+class _Nothing:
+    """Stands for the extension where it is not built: declines every call."""
+
+    attend = select = copy = alloc = release = fork = compact = staticmethod(lambda *args: None)
+
+
+_calls = None
+
+
+def _torch_calls():
+    global _calls
+    _calls = _lib.torch_calls() or _Nothing
+    return _calls
+
+
+def _made(result, name: str) -> bool:
+    """Whether the extension made the call; raises the library's error."""
+    if result is None:
+        return False
+    if type(result) is int:
+        raise _lib.GdnError(name, result, _lib.strerror(result))
+    return True
+
+
+# Through ctypes: the common case of each check is one chain of comparisons, and the stream
+# and device come from torch's cheapest accessors (72 ns against 2.2 us for
+# torch.cuda.current_stream).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -113,6 +140,10 @@ def paged_attention_decode(
     token is seen even when its page is bad, but not stored.  The page of a sequence's last
     token must not be shared.  C entry: ``gdn_paged_attention_decode``.
     """
+    made = (_calls or _torch_calls()).attend(q, k_cache, v_cache, block_tables, seq_lens, k, v, scale,
+                                            window, num_sinks, output, bad_index_count)
+    if _made(made, "gdn_paged_attention_decode"):
+        return made
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[1] != 1:
         raise ValueError("q must be 4-D [B, 1, heads, head_dim]")
     B, _, HQ, D = q.shape
@@ -187,6 +218,9 @@ def beam_select(
     a NaN or +inf) are never chosen; places left over get -1, -1, -inf.  At most 64 beams and
     64 selected.  C entry: ``gdn_beam_select``.
     """
+    made = (_calls or _torch_calls()).select(logits, scores, num_selected, finished, eos_token)
+    if _made(made, "gdn_beam_select"):
+        return made
     if not isinstance(logits, torch.Tensor) or logits.dim() != 3:
         raise ValueError("logits must be 3-D [B, beams, vocab]")
     B, K, V = logits.shape
@@ -272,6 +306,9 @@ def copy_pages(pools: Pools, src, dst, bad_index_count=None) -> None:
     index skips its pair, one >= num_pages does too and is counted in ``bad_index_count``.
     C entry: ``gdn_copy_pages``.
     """
+    made = (_calls or _torch_calls()).copy(pools, src, dst, bad_index_count)
+    if _made(made, "gdn_copy_pages"):
+        return
     p = _PoolArrays(pools)
     if p.count == 0:
         return
@@ -290,6 +327,9 @@ def alloc_pages(refcounts, need) -> torch.Tensor:
     lowest free pages of ``refcounts`` [num_pages] int32 in order (their count becomes 1);
     -1 where nothing is needed or no page is left.  A page is free when its count is <= 0.
     C entry: ``gdn_alloc_pages``."""
+    made = (_calls or _torch_calls()).alloc(refcounts, need)
+    if _made(made, "gdn_alloc_pages"):
+        return made[0]
     P, dev = _check_refcounts(refcounts)
     if not isinstance(need, torch.Tensor) or need.dim() != 1:
         raise ValueError("need must be a 1-D bool tensor")
@@ -307,6 +347,9 @@ def free_pages(refcounts, pages, bad_index_count=None) -> None:
     contiguous: block-table rows go in as they are, negative entries are skipped).  Entries
     >= num_pages and entries of pages without a reference left are counted in
     ``bad_index_count`` and change nothing.  C entry: ``gdn_free_pages``."""
+    made = (_calls or _torch_calls()).release(refcounts, pages, bad_index_count)
+    if _made(made, "gdn_free_pages"):
+        return
     P, dev = _check_refcounts(refcounts)
     _need(pages, "pages", _I32, None, dev)
     _check_counter(bad_index_count, dev)
@@ -327,6 +370,10 @@ def fork_pages(block_tables, seq_lens, parents, refcounts, page_size: int, pools
     page was left (its entry becomes -1).  Entries behind a row's tokens are -1.
     C entry: ``gdn_fork_pages``.
     """
+    made = (_calls or _torch_calls()).fork(block_tables, seq_lens, parents, refcounts, page_size, pools,
+                                          bad_index_count)
+    if _made(made, "gdn_fork_pages"):
+        return made
     P, dev = _check_refcounts(refcounts)
     if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
         raise ValueError("block_tables must be 2-D [rows, width]")
@@ -358,6 +405,9 @@ def compact_pages(refcounts, block_tables=None, pools: Pools = ()) -> Tuple[torc
     updated in place.  Returns ``(remap [num_pages] int32, num_live [1] int32)``: each live
     page's new number, -1 for a free one.  C entry: ``gdn_compact_pages``.
     """
+    made = (_calls or _torch_calls()).compact(refcounts, block_tables, pools)
+    if _made(made, "gdn_compact_pages"):
+        return made
     P, dev = _check_refcounts(refcounts)
     entries = 0
     if block_tables is not None:
