@@ -453,12 +453,17 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 // in the sorted lists instead.
 
 constexpr int kMergeList = 1024, kHeld = 8;
+constexpr int kTokenBits = 26;   // of the vocabulary (checked on the host)
 
-struct MergeItem {
-  unsigned long long score;      // of the 64-bit score, in an order-preserving form
-  unsigned long long key;        // of its logit and token; ~0 for a finished beam's one
-  int beam;
+// A candidate as a 128-bit number that orders like it: the score's bits, then the lower beam,
+// then the larger logit, then the lower token.
+struct __align__(16) MergeItem {
+  unsigned long long hi, lo;
 };
+__device__ __forceinline__ bool better(const MergeItem& a, const MergeItem& b) {
+  return ((static_cast<unsigned __int128>(a.hi) << 64) | a.lo) >
+         ((static_cast<unsigned __int128>(b.hi) << 64) | b.lo);
+}
 
 __device__ __forceinline__ unsigned long long ordered(double x) {
   const unsigned long long u = __double_as_longlong(x + 0.0);   // -0 and +0 are equal
@@ -466,6 +471,11 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
 }
 __device__ __forceinline__ double from_ordered(unsigned long long o) {
   return __longlong_as_double(o >> 63 ? o & 0x7fffffffffffffffull : ~o);
+}
+__device__ __forceinline__ MergeItem make_item(double score, int beam, unsigned long long key) {
+  constexpr unsigned long long tokens = (1ull << kTokenBits) - 1;
+  return MergeItem{ordered(score), static_cast<unsigned long long>(kMaxBeams - 1 - beam) << 58 |
+                                       (key >> 32) << kTokenBits | (key & tokens)};
 }
 
 // ln(t) for t >= 1: the fraction's logarithm in fp32 (6e-8), the exponent's in 64 bits
@@ -476,30 +486,31 @@ __device__ __forceinline__ double ln_sum(double t) {
   return e * 0.69314718055994530942 + static_cast<double>(logf(static_cast<float>(f)));
 }
 
-// sum over a group of 8 lanes; groups of one warp may have left the loop
-template <typename T> __device__ __forceinline__ T sum8(T x) {
-  const uint32_t mask = 0xffu << (threadIdx.x & 24);
+// over a group of N lanes; other groups of the warp may have left the loop
+template <int N, typename T> __device__ __forceinline__ T group_sum(T x) {
+  const uint32_t mask = ((1u << N) - 1) << (threadIdx.x & (32 - N));
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
+  for (int o = N / 2; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
   return x;
 }
-__device__ __forceinline__ float max8(float x) {
-  const uint32_t mask = 0xffu << (threadIdx.x & 24);
+template <int N> __device__ __forceinline__ float group_max(float x) {
+  const uint32_t mask = ((1u << N) - 1) << (threadIdx.x & (32 - N));
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(mask, x, o));
+  for (int o = N / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(mask, x, o));
   return x;
 }
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
   __shared__ double lse[kMaxBeams], cum[kMaxBeams], bound;
+  __shared__ float least[kMaxBeams];       // logits below are below the bound, by beam
   __shared__ unsigned long long head[kHeadItems];
   __shared__ MergeItem item[kMergeList];
-  __shared__ int count, alive;
+  __shared__ int count;
   __shared__ bool done[kMaxBeams];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int per_beam = p.slices * p.n, lists = p.K * p.slices, total = lists * p.n;
   if (tid == 0) {
-    count = alive = 0;
+    count = 0;
     bound = -INFINITY;
   }
   if (tid < p.K) {
@@ -521,25 +532,27 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   }
   const int depth = (p.n + lists - 1) / lists, items = min(lists * depth, kHeadItems);
   const unsigned long long head_key = tid < items ? all[tid % lists * p.n + tid / lists] : 0;
-  const int i8 = tid / 8;
+  const int i8 = tid / 8, s8 = tid % 8;
   if (i8 < p.K) {
     double l = NAN;                     // not finite: a beam without candidates of its own
     const bool on = !done[i8] && isfinite(cum[i8]);
     const float2* sums = p.sums + (static_cast<long long>(b) * p.K + i8) * p.slices;
-    float m = -INFINITY;
+    const float2 first = on && s8 < p.slices ? sums[s8] : make_float2(-INFINITY, 0.f);
+    float m = first.x;
     if (on)
-      for (int s = tid % 8; s < p.slices; s += 8) m = fmaxf(m, sums[s].x);
-    m = max8(m);
-    double t = 0.0;
+      for (int s = s8 + 8; s < p.slices; s += 8) m = fmaxf(m, sums[s].x);
+    m = group_max<8>(m);
+    auto term = [&](float2 ms) {
+      return ms.x > -INFINITY || isnan(ms.y)
+                 ? static_cast<double>(ms.y) * static_cast<double>(exp2_fast((ms.x - m) * kLog2e))
+                 : 0.0;
+    };
+    double t = term(first);
     if (on)
-      for (int s = tid % 8; s < p.slices; s += 8) {
-        const float2 ms = sums[s];
-        if (ms.x > -INFINITY || isnan(ms.y))
-          t += static_cast<double>(ms.y) * static_cast<double>(exp2f((ms.x - m) * kLog2e));
-      }
-    t = sum8(t);
+      for (int s = s8 + 8; s < p.slices; s += 8) t += term(sums[s]);
+    t = group_sum<8>(t);
     if (on && isfinite(m) && t >= 0.5 && t < 1e300) l = m + ln_sum(t);
-    if (tid % 8 == 0) lse[i8] = l;
+    if (s8 == 0) lse[i8] = l;
   }
   __syncthreads();
   auto score_of = [&](int i, unsigned long long k) {
@@ -551,57 +564,61 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     head[tid] = ordered(head_key && isfinite(lse[i]) ? score_of(i, head_key) : -INFINITY);
   }
   __syncthreads();
-  __syncthreads();
-  // eight threads count for one
-  for (int f = tid / 8; f < items; f += kMergeThreads / 8) {
+  // four threads count for one
+  for (int f = tid / 4; f < items; f += kMergeThreads / 4) {
     const unsigned long long sc = head[f];
     int rank = 0;
-    for (int o = tid % 8; o < items; o += 8) rank += (head[o] > sc) | ((head[o] == sc) & (o < f));
-    rank = sum8(rank);
+#pragma unroll 4
+    for (int o = tid % 4; o < items; o += 4) rank += (head[o] > sc) | ((head[o] == sc) & (o < f));
+    rank = group_sum<4>(rank);
     if (rank == p.n - 1) bound = from_ordered(sc);
   }
   __syncthreads();
   const double low = bound;
-  int valid = 0;
+  // below this logit no score reaches the bound: rounded down, far below what rounding the
+  // score in 64 bits can move; NaN for a beam without candidates, -inf without a bound
+  if (tid < p.K) {
+    const double x = low - cum[tid] + lse[tid];
+    least[tid] = !isfinite(lse[tid]) ? NAN
+                 : !isfinite(x)      ? -INFINITY
+                                     : static_cast<float>(x - 1e-6 * (1.0 + fabs(x)));
+  }
+  __syncthreads();
   auto take = [&](int f, unsigned long long k) {
     const int i = f / per_beam;
-    if (k == 0 || !isfinite(lse[i])) return;
-    ++valid;
+    if (k == 0 || !(key_logit(k) >= least[i])) return;
     const double sc = score_of(i, k);
     if (!(sc >= low)) return;
     const int at = next_place(&count);
-    if (at < kMergeList) item[at] = MergeItem{ordered(sc), k, i};
+    if (at < kMergeList) item[at] = make_item(sc, i, k);
   };
 #pragma unroll
   for (int u = 0; u < kHeld; ++u)
     if (u * kMergeThreads + tid < total) take(u * kMergeThreads + tid, held[u]);
   for (int f = kHeld * kMergeThreads + tid; f < total; f += kMergeThreads) take(f, all[f]);
-  if (tid < p.K && done[tid] && isfinite(cum[tid])) {
-    ++valid;
-    if (cum[tid] >= low) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kMergeList) item[at] = MergeItem{ordered(cum[tid]), ~0ull, tid};
-    }
+  if (tid < p.K && done[tid] && isfinite(cum[tid]) && cum[tid] >= low) {
+    const int at = next_place(&count);
+    if (at < kMergeList) item[at] = make_item(cum[tid], tid, 0);
   }
-  if (valid) atomicAdd(&alive, valid);
   __syncthreads();
-  auto place = [&](int rank, double sc, int i, unsigned long long k) {
+  // (rank, score, beam, token); with a bound there are n candidates at least
+  auto place = [&](int rank, double sc, int i, int token) {
     const long long at = static_cast<long long>(b) * p.n + rank;
-    p.tokens[at] = k == ~0ull ? p.eos : key_token(k);
+    p.tokens[at] = done[i] ? p.eos : token;
     p.parents[at] = i;
     p.out_scores[at] = static_cast<float>(sc);
   };
+  const int alive = low > -INFINITY ? p.n : count;
   if (count <= kMergeList) {
-    for (int f = tid / 8; f < count; f += kMergeThreads / 8) {
+    for (int f = tid / 4; f < count; f += kMergeThreads / 4) {
       const MergeItem me = item[f];
       int rank = 0;
-      for (int o = tid % 8; o < count; o += 8) {
-        const MergeItem it = item[o];
-        rank += (it.score > me.score) |
-                ((it.score == me.score) & ((it.beam < me.beam) | ((it.beam == me.beam) & (it.key > me.key))));
-      }
-      rank = sum8(rank);
-      if (rank < p.n && tid % 8 == 0) place(rank, from_ordered(me.score), me.beam, me.key);
+#pragma unroll 4
+      for (int o = tid % 4; o < count; o += 4) rank += better(item[o], me);
+      rank = group_sum<4>(rank);
+      if (rank < p.n && tid % 4 == 0)
+        place(rank, from_ordered(me.hi), kMaxBeams - 1 - static_cast<int>(me.lo >> 58),
+              static_cast<int>(0xffffffffu - (static_cast<uint32_t>(me.lo) | ~((1u << kTokenBits) - 1))));
     }
   } else {
     // better ones in every list: higher scores, and equal ones of lower beams or, within the
@@ -637,7 +654,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
           rank += lo;
         }
       }
-      if (rank < p.n) place(rank, sc, i, k);
+      if (rank < p.n) place(rank, sc, i, key_token(k));
     }
   }
   for (int r = alive + tid; r < p.n; r += kMergeThreads) {
@@ -693,7 +710,7 @@ int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch, int64_t
   if (!aligned(logits, dtype == GDN_DTYPE_FP32 ? 4 : 2) || !aligned(scores, 4) || !aligned(tokens, 4) ||
       !aligned(parents, 4) || !aligned(new_scores, 4) || !aligned(workspace, 16))
     return GDN_ERR_ALIGN;
-  if (V > (1 << 26)) return GDN_ERR_SHAPE;           // keeps the slices of a row below 2^16
+  if (V > 1 << kTokenBits) return GDN_ERR_SHAPE;     // also keeps the slices of a row below 2^16
   if (workspace_bytes < gdn_beam_select_workspace_bytes(B, K, V, n)) return GDN_ERR_SHAPE;
   BeamArgs p{};
   p.logits = logits; p.scores = scores; p.finished = finished; p.tokens = tokens;
