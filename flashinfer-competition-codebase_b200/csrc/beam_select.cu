@@ -25,7 +25,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBatch = 4;        // 16-byte vectors of logits a thread takes at a time
 constexpr int kList = 1024;      // vectors, then candidates, that a slice gathers
 constexpr int kMergeThreads = 512;
-constexpr int kHeadItems = 256;  // of the merge's bound
+constexpr int kHeadItems = 256;  // of the merge's bound, at most 256
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct BeamArgs {
@@ -39,6 +39,7 @@ struct BeamArgs {
   float2* sums;               // workspace [rows, slices]: m, sum exp(x - m)
   long long stride_batch, stride_beam;
   int B, K, V, n, eos, slices;
+  uint32_t per_mul, per_shift;   // division by slices n
 };
 
 template <typename T> __device__ __forceinline__ float to_f(T x);
@@ -455,16 +456,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 constexpr int kMergeList = 1024, kHeld = 8;
 constexpr int kTokenBits = 26;   // of the vocabulary (checked on the host)
 
-// A candidate as a 128-bit number that orders like it: the score's bits, then the lower beam,
-// then the larger logit, then the lower token.
+// A candidate as two numbers that order like it: the score's bits; the lower beam, then the
+// larger logit, then the lower token.
 struct __align__(16) MergeItem {
   unsigned long long hi, lo;
 };
-__device__ __forceinline__ bool better(const MergeItem& a, const MergeItem& b) {
-  return ((static_cast<unsigned __int128>(a.hi) << 64) | a.lo) >
-         ((static_cast<unsigned __int128>(b.hi) << 64) | b.lo);
-}
-
 __device__ __forceinline__ unsigned long long ordered(double x) {
   const unsigned long long u = __double_as_longlong(x + 0.0);   // -0 and +0 are equal
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
@@ -561,7 +557,9 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   // a slice that wrote nothing (its beam is finished or dead) leaves stale keys: lse says so
   if (tid < items) {
     const int i = tid % lists / p.slices;
-    head[tid] = ordered(head_key && isfinite(lse[i]) ? score_of(i, head_key) : -INFINITY);
+    // all different: the last 8 bits are the place instead of the score's, which rounds down
+    head[tid] = (ordered(head_key && isfinite(lse[i]) ? score_of(i, head_key) : -INFINITY) & ~255ull) |
+                static_cast<unsigned>(tid);
   }
   __syncthreads();
   // four threads count for one
@@ -569,9 +567,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     const unsigned long long sc = head[f];
     int rank = 0;
 #pragma unroll 4
-    for (int o = tid % 4; o < items; o += 4) rank += (head[o] > sc) | ((head[o] == sc) & (o < f));
+    for (int o = tid % 4; o < items; o += 4) rank += head[o] > sc;
     rank = group_sum<4>(rank);
-    if (rank == p.n - 1) bound = from_ordered(sc);
+    if (rank == p.n - 1) {
+      const double low = from_ordered(sc & ~255ull);
+      bound = isfinite(low) ? low : -INFINITY;
+    }
   }
   __syncthreads();
   const double low = bound;
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   }
   __syncthreads();
   auto take = [&](int f, unsigned long long k) {
-    const int i = f / per_beam;
+    const int i = static_cast<int>(div_by(f, p.per_mul, p.per_shift));
     if (k == 0 || !(key_logit(k) >= least[i])) return;
     const double sc = score_of(i, k);
     if (!(sc >= low)) return;
@@ -612,9 +613,15 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   if (count <= kMergeList) {
     for (int f = tid / 4; f < count; f += kMergeThreads / 4) {
       const MergeItem me = item[f];
-      int rank = 0;
+      int rank = 0, same = 0;
 #pragma unroll 4
-      for (int o = tid % 4; o < count; o += 4) rank += better(item[o], me);
+      for (int o = tid % 4; o < count; o += 4) {
+        const unsigned long long hi = item[o].hi;
+        rank += hi > me.hi;
+        same += hi == me.hi;
+      }
+      if (group_sum<4>(same) > 1)        // equal scores: by beam, logit, token
+        for (int o = tid % 4; o < count; o += 4) rank += item[o].hi == me.hi && item[o].lo > me.lo;
       rank = group_sum<4>(rank);
       if (rank < p.n && tid % 4 == 0)
         place(rank, from_ordered(me.hi), kMaxBeams - 1 - static_cast<int>(me.lo >> 58),
@@ -720,6 +727,7 @@ int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch, int64_t
   p.sums = reinterpret_cast<float2*>(p.keys + static_cast<size_t>(B) * K * p.slices * n);
   p.stride_batch = stride_batch; p.stride_beam = stride_beam;
   p.B = B; p.K = K; p.V = V; p.n = n; p.eos = eos_token;
+  div_constants(static_cast<uint32_t>(p.slices * n), p.per_mul, p.per_shift);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == GDN_DTYPE_BF16) return launch<__nv_bfloat16>(p, st);
   if (dtype == GDN_DTYPE_FP16) return launch<__half>(p, st);
