@@ -85,9 +85,7 @@ template <int D> struct Shape {
   static constexpr int kResident = D == 256 ? 1 : 2;
 };
 
-// units of one of sequence b's rows in the line
 template <int kBlock> __device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
-  if (!p.cut) return 1;
   const int vis = sequence(p, p.lens[b]).vis;
   return vis > 0 ? (vis + kBlock - 1) / kBlock : 1;
 }
@@ -114,6 +112,17 @@ template <int kBlock> __device__ Share my_share(const AttnArgs& p) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, rows = p.HKV * p.tiles;
   long long base = 0, first = 0;
   int n = 0;
+  Share s;
+  s.start = s.end = 0;
+  if (!p.cut) {                          // whole rows: the lengths do not matter
+    s.total = static_cast<long long>(p.B) * rows;
+    s.count = s.total < p.grid ? s.total : p.grid;
+    if (blockIdx.x >= s.count) return s;
+    s.start = share_start(blockIdx.x, s.total, s.count);
+    s.end = share_start(blockIdx.x + 1, s.total, s.count);
+    s.before = s.b = static_cast<int>(s.start / rows);
+    return s;
+  }
   auto scan = [&](int b0) {              // sequences b0 ...: n and first of b0 + tid
     n = b0 + tid < p.B ? blocks_of<kBlock>(p, b0 + tid) : 0;
     long long x = n;
@@ -133,10 +142,8 @@ template <int kBlock> __device__ Share my_share(const AttnArgs& p) {
     }
   };
   for (int b0 = 0; b0 < p.B; b0 += N) scan(b0);
-  Share s;
   s.total = base * rows;
   s.count = s.total < p.grid ? s.total : p.grid;
-  s.start = s.end = 0;
   if (blockIdx.x >= s.count) return s;
   s.start = share_start(blockIdx.x, s.total, s.count);
   s.end = share_start(blockIdx.x + 1, s.total, s.count);
@@ -271,8 +278,9 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     const int tok = token_of(k);
     return tok < 0 ? -1 : __ldg(p.tables + f_b * p.table_stride + div_by(tok, p.page_mul, p.page_shift));
   };
-  // Turns to the row at line position `at` (of sequence f_b, whose tokens are `len`).
-  auto open = [&](Row& r, int len) {
+  // Turns to the row at line position `at` (of sequence f_b, whose tokens are `len`); `early`:
+  // the page of this lane's token when that does not depend on len, or -1.
+  auto open = [&](Row& r, int len, int early) {
     f = sequence(p, len);
     const int nb = f.vis > 0 ? (f.vis + S::kBlock - 1) / S::kBlock : 1;
     const long long in_seq = at - before * rows, left = share.end - at;
@@ -284,7 +292,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     r.row = f_row;
     r.blocks = f_k1 - f_k;
     r.whole = f_k == 0 && f_k1 == nb;
-    page = page_of(f_k);
+    page = early >= 0 && token_of(f_k) >= 0 ? early : page_of(f_k);
     if (tid == 0) {
       if (f_row == 0 && f_k == 0 && p.bad != nullptr && len > f.len) atomicAdd(p.bad, 1);
       if (p.cut && (p.by_row ? f_k1 == nb : at == share.start)) {
@@ -377,7 +385,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     if (f_k == f_k1 && !ahead_row && at < share.end) {
       const bool same = f_row + 1 < rows;                     // the sequence has more rows
       f_b += same ? 0 : 1;
-      open(next, same ? p.lens[f_b] : len_next);
+      open(next, same ? p.lens[f_b] : len_next, -1);
       ahead_row = true;
     }
   };
@@ -400,8 +408,21 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     }
   };
 
-  open(row, p.lens[f_b]);
-  load_queries();
+  {
+    // the first row: what does not wait for its length is loaded beside it
+    const int len = p.lens[f_b];
+    int early = -1;
+    if (!p.cut) {
+      row.b = f_b;
+      row.row = static_cast<int>(at - before * rows);
+      load_queries();
+      const int j = warp * S::kTile + (lane & (S::kTile - 1));
+      if (p.window == 0 && j < p.width * p.page_size)
+        early = __ldg(p.tables + f_b * p.table_stride + div_by(j, p.page_mul, p.page_shift));
+    }
+    open(row, len, early);
+    if (p.cut) load_queries();
+  }
   fetch();
   advance();
   fetch();
@@ -663,11 +684,10 @@ int heads_of(int group) { return group <= 8 ? 8 : 16; }
 int block_of(int D) { return D == 64 ? Shape<64>::kBlock : D == 128 ? Shape<128>::kBlock : Shape<256>::kBlock; }
 int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
 
-// Rows of up to 4 blocks are not cut, and of up to 8 where there is a row for every CTA: one
-// CTA takes such a row in less than the cut's partial sums and the join cost.  Not cut / cut:
-// 1 row of 100 tokens of 128 dims 5.8 / 7.1 us, of 512 tokens 10.7 / 7.1 us; 512 rows of
-// 256 tokens 14.8 / 22.1 us, of 500 tokens 22.4 / 30.5 us.
-constexpr int kWhole = 4, kWholeMany = 8;
+// Rows are not cut where that leaves no CTA more than about 2.5 blocks over an even share:
+// less than the cut's partial sums and the join cost.  Not cut / cut: 1 row of 100 tokens of
+// 128 dims 5.8 / 7.1 us, of 512 tokens 10.7 / 7.1 us; 512 rows of 256 tokens 14.8 / 22.1 us,
+// of 500 tokens 22.4 / 30.5 us.
 
 struct Plan {
   long long rows, grid;      // rows of a call; CTAs: what the GPU holds at once, or fewer
@@ -681,7 +701,8 @@ Plan plan_of(int B, int HQ, int HKV, int D, long long max_tokens) {
   q.rows = static_cast<long long>(B) * HKV * ((HQ / HKV + heads - 1) / heads);
   const long long nb = max_tokens > 0 ? (max_tokens + block_of(D) - 1) / block_of(D) : 1;
   const long long most = static_cast<long long>(kSMs) * resident(D);
-  q.split = nb > (q.rows >= most ? kWholeMany : kWhole);
+  const long long waves = (q.rows + most - 1) / most;
+  q.split = 2 * nb * (waves * most - q.rows) > 5 * most;
   const long long units = q.rows * (q.split ? nb : 1);
   q.grid = units < most ? units : most;
   q.cut = static_cast<size_t>(q.rows <= q.grid ? q.rows : q.grid);
