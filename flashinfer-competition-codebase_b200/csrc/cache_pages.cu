@@ -14,6 +14,8 @@
 
 #include <string.h>
 
+#include <algorithm>
+
 #include "serving_common.cuh"
 
 namespace {
@@ -181,20 +183,35 @@ struct MoveArgs {
   const int32_t* dst;
   const int32_t* count;            // device count of pairs, or null: n
   int n;
+  // compaction's last steps, or remap null
   int32_t* tables;                 // entries to rewrite through remap, or null
-  const int32_t* remap;            // [num_pages]
+  int32_t* remap;                  // [num_pages], the k-th mover's as -2 - k
+  int32_t* refcounts;              // [num_pages]
   long long entries;
 };
 
 template <typename U>
 __global__ void __launch_bounds__(kThreads) move_pages_kernel(const __grid_constant__ MoveArgs p) {
   grid_wait();                     // the plan is the kernel before
-  const long long step = static_cast<long long>(gridDim.x) * kThreads;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < p.entries; i += step) {
-    const int page = p.tables[i];
-    if (page >= 0 && page < p.pools.num_pages) p.tables[i] = p.remap[page];
-  }
   const long long n = p.count ? *p.count : p.n;
+  if (p.remap) {
+    // a mover's entry is read by the tables' threads while its own thread replaces it: both
+    // values lead to the same page
+    const long long step = static_cast<long long>(gridDim.x) * kThreads;
+    const long long me = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x;
+    for (long long k = me; k < n; k += step) {
+      const int s = p.src[k], d = p.dst[k];
+      p.refcounts[d] = p.refcounts[s];
+      p.refcounts[s] = 0;
+      __stcg(p.remap + s, d);
+    }
+    for (long long i = me; i < p.entries; i += step) {
+      const int page = p.tables[i];
+      if (page < 0 || page >= p.pools.num_pages) continue;
+      const int to = __ldcg(p.remap + page);
+      p.tables[i] = to <= -2 ? p.dst[-2 - to] : to;
+    }
+  }
   long long item = blockIdx.x;
   for (int pool = 0; pool < p.pools.count; ++pool) {
     const long long vecs = p.pools.bytes[pool] / static_cast<int>(sizeof(U));
@@ -408,12 +425,10 @@ struct CompactArgs {
 // Each thread looks after a run of neighbouring pages, four at a time.  With before(i) the
 // live pages before page i and L all of them, a free page i < L is hole number
 // i - before(i), and a live page i >= L is mover number before(i) - before(L); there are
-// L - before(L) of either.  The k-th of each are paired through shared memory, or through the
-// workspace where there are more than it holds.
-constexpr int kPaired = 4096;
-
+// L - before(L) of either.  Pairing the k-th of each, with its scattered writes, is left to
+// the moving kernel's many CTAs (it cost this one CTA 4.5 us of 9).
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactArgs p) {
-  __shared__ int before_live, hole[kPaired];
+  __shared__ int before_live;
   grid_trigger();
   const int groups = (p.P + 3) / 4, run = (groups + kPlanThreads - 1) / kPlanThreads;
   const int g0 = min(static_cast<int>(threadIdx.x) * run, groups), g1 = min(g0 + run, groups);
@@ -454,11 +469,11 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
       const int i = 4 * g + u;
       const bool on = cs[u] > 0;
       to[u] = on ? i : -1;
-      if (!on && i < live) {       // live <= P: the padding is no hole
-        const int k = i - before;
-        p.dst[k] = i;
-        if (k < kPaired) hole[k] = i;
+      if (on && i >= live) {
+        to[u] = -2 - (before - kept);
+        p.src[before - kept] = i;
       }
+      if (!on && i < live) p.dst[i - before] = i;   // live <= P: the padding is no hole
       before += on;
     }
     if (wide && 4 * g + 4 <= p.P && (reinterpret_cast<uintptr_t>(p.remap) & 15) == 0) {
@@ -467,24 +482,6 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (4 * g + u < p.P) p.remap[4 * g + u] = to[u];
-    }
-  }
-  __syncthreads();
-  // the movers: only counts of pages before `live` change here, and those are not read
-  before = first;
-  for (int g = max(g0, live / 4); g < g1; ++g) {
-    const int4 c = counts(g);
-    const int* cs = &c.x;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = 4 * g + u;
-      if (i == live) before = kept;
-      if (i < live || cs[u] <= 0) continue;
-      const int k = before++ - kept, d = k < kPaired ? hole[k] : p.dst[k];
-      p.src[k] = i;
-      p.remap[i] = d;
-      p.refcounts[d] = cs[u];
-      p.refcounts[i] = 0;
     }
   }
   if (threadIdx.x == 0) {
@@ -687,16 +684,17 @@ int gdn_compact_pages(int32_t* refcounts, int num_pages, int32_t* block_tables,
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
-  if (num_pools == 0 && table_entries == 0) return GDN_OK;
   m.tables = block_tables;
   m.entries = table_entries;
   m.remap = remap;
+  m.refcounts = refcounts;
   m.src = p.src;
   m.dst = p.dst;
   m.count = p.count;
-  const unsigned grid = num_pools > 0 ? grid_for(m.pools, unit, static_cast<long long>(half), 8)
-                                      : static_cast<unsigned>(table_entries < 2 * kSMs * kThreads
-                                            ? (table_entries + kThreads - 1) / kThreads : 2 * kSMs);
+  const long long small = std::max(static_cast<long long>(table_entries), static_cast<long long>(half));
+  const unsigned grid = num_pools > 0
+                            ? grid_for(m.pools, unit, static_cast<long long>(half), 8)
+                            : static_cast<unsigned>(std::min((small + kThreads - 1) / kThreads, 2ll * kSMs));
   return launch_moves(m, unit, grid, st) == cudaSuccess
              ? GDN_OK : GDN_ERR_LAUNCH;
 }
