@@ -94,6 +94,11 @@ template <typename T> struct Vec {
 
 // ------------------------------------------------------------------ one slice of a row
 //
+// A row's slices are counted in vectors of 16 bytes from its first token, and a row that need
+// not begin on a 16-byte boundary is read in words of 32 bits (64 x 8 rows of 151936 bf16
+// logits: 55 us instead of 49): equal rows get equal sums, bit for bit, wherever they lie, so
+// that equal beams tie.
+//
 // One pass over the slice.  Every thread keeps its own running maximum and its sum of
 // exponentials relative to it, so the loop has no barrier; its next batch of vectors is in
 // flight while it works on one.  The first batch is a sample spread over the slice: with
@@ -101,9 +106,15 @@ template <typename T> struct Vec {
 // at or above it.  Vectors that reach T are set aside as they are; at the end the n-th
 // largest of their maxima is a sharper bound, and what reaches that is ranked.
 //
-// Bound: HBM for fp32; for 16-bit logits the exponentials come near it (12.3 logits a clock
-// and SM at the measured copy rate, of 16 exponentials), so an element costs one unpack,
-// one fused multiply-add, one exponential, one addition and parts of packed maxima.
+// Bound: the issue of instructions.  The exponentials alone come near HBM for 16-bit logits
+// (12.3 logits a clock and SM at the measured copy rate, of 16 exponentials), so an element
+// costs one unpack, one exponential, half of a packed multiply-add and of a packed addition,
+// and parts of packed maxima: 94 instructions for a vector of eight with all that is set
+// aside.  64 x 8 rows of 151936 bf16 logits, a tenth finished: 42 us (140 MB, 3.3 TB/s, 28.7
+// million warp instructions; a copy's rate would read them in 21).  8 x 32 rows of 50257 fp32, a
+// quarter finished: 15 us (39 MB, 2.6 TB/s; 14 with rows padded to begin on 16 bytes).
+// Tried there without gain: three to eight CTAs an SM (41 to 72 us), batches of 2 and 8, a ring
+// of asynchronous copies through shared memory (50), places by ballots (55).
 
 struct SliceShared {
   uint4 vec[kList];                // vectors that reach T
@@ -191,7 +202,8 @@ __device__ void write_ranked(const unsigned long long* list, int c, int n, unsig
   for (int i = c + threadIdx.x; i < n; i += kThreads) out[i] = 0;
 }
 
-template <typename T>
+// kShift: rows need not begin on a 16-byte boundary.
+template <typename T, bool kShift>
 __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs p) {
   using V = Vec<T>;
   constexpr int E = V::kN;
@@ -203,38 +215,68 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   const bool done = p.finished != nullptr && p.finished[row];
   if (done | !isfinite(p.scores[row])) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + b * p.stride_batch + i * p.stride_beam;
-  // the row as aligned 16-byte vectors; vector c holds tokens c E - mis ...; the first and the
-  // last may be partial and are handled one by one
-  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int vecs = (p.V + mis + E - 1) / E;
+  // vector c holds tokens c E ...; the row's end is read token by token
+  const int vecs = (p.V + E - 1) / E, whole = p.V / E;
   const int each = vecs / p.slices, more = vecs - each * p.slices;   // the first `more` get one more
   const int v0 = slice * each + min(slice, more), v1 = v0 + each + (slice < more ? 1 : 0);
-  const int lo = v0 == 0 && mis ? 1 : v0, hi = v1 == vecs && (p.V + mis) % E ? v1 - 1 : v1;
-  const uint4* base = reinterpret_cast<const uint4*>(x - mis);
-  // batch j of thread tid: whole vectors lo + (j + k batches) 256 + tid, k < kBatch
-  const int batches = max(1, (hi - lo + kThreads * kBatch - 1) / (kThreads * kBatch));
-  V none;
-  {
-    T inf[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) inf[e] = T(-INFINITY);
-    none.u = *reinterpret_cast<uint4*>(inf);
-  }
-  auto load = [&](V (&v)[kBatch], int j) {
+  // kShift with 16-bit tokens: the row begins in the middle of a word, so that the first and
+  // the last word read hold a token outside the row beside one of its own
+  const bool half = sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(x) & 2);
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(x - (half ? 1 : 0));
+  // batch j of thread tid: vectors v0 + (j + k batches) 256 + tid, k < kBatch
+  const int batches = (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch);
+  // what is in flight: words as they lie, put in place when their turn comes
+  struct Raw {
+    uint32_t w[kShift && E == 8 ? 5 : 4];
+  };
+  // -inf throughout
+  constexpr uint32_t none = std::is_same_v<T, float> ? 0xff800000u
+                            : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+  auto load = [&](Raw (&raw)[kBatch], int j) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int c = lo + (j + k * batches) * kThreads + tid;
-      v[k] = none;
-      if (c < hi) v[k].u = __ldcs(base + c);
+      const int c = v0 + (j + k * batches) * kThreads + tid;
+      uint32_t (&w)[sizeof(Raw) / 4] = raw[k].w;
+#pragma unroll
+      for (int i = 0; i < sizeof(Raw) / 4; ++i) w[i] = none;
+      if (c < min(v1, whole)) {
+        if constexpr (!kShift) {
+          const uint4 u = __ldcs(reinterpret_cast<const uint4*>(x) + c);
+          w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = __ldg(words + 4 * c + i);
+          if constexpr (E == 8)
+            if (half) w[4] = __ldg(words + 4 * c + 4);
+        }
+      } else if (c < v1) {
+        T end[sizeof(Raw) / sizeof(T)];
+        const int first = c * E - (half ? 1 : 0);
+#pragma unroll 1
+        for (int e = 0; e < sizeof(Raw) / sizeof(T); ++e)
+          end[e] = first + e >= c * E && first + e < p.V ? x[first + e] : T(-INFINITY);
+#pragma unroll
+        for (int i = 0; i < sizeof(Raw) / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(end)[i];
+      }
     }
   };
+  auto vector = [&](const Raw& raw) {
+    uint4 u = make_uint4(raw.w[0], raw.w[1], raw.w[2], raw.w[3]);
+    if constexpr (kShift && E == 8)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) (&u.x)[i] = __funnelshift_r(raw.w[i], raw.w[i + 1], half ? 16 : 0);
+    return V{u};
+  };
   V v[kBatch];
-  load(v, 0);
+  Raw next[kBatch];
+  load(next, 0);
   if (tid == 0) {
     sh.count = sh.keys = 0;
     sh.bound = -INFINITY;
   }
   float m = -INFINITY;           // this thread's largest logit
+#pragma unroll
+  for (int k = 0; k < kBatch; ++k) v[k] = vector(next[k]);
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) m = fmaxf(m, v[k].largest());
   {
@@ -263,32 +305,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     sums.scale(f);
     c0 = c1;
   };
-  if (lo != v0 || hi != v1) {    // partial vectors: two threads of the first and last slice
-    const int c = tid == 0 && lo != v0 ? v0 : tid == 32 && hi != v1 ? v1 - 1 : -1;
-    if (c >= 0) {
-      V w = none;
-      T tmp[E];
-      *reinterpret_cast<uint4*>(tmp) = none.u;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int t = c * E - mis + e;
-        if (t >= 0 && t < p.V) tmp[e] = x[t];
-      }
-      w.u = *reinterpret_cast<uint4*>(tmp);
-      if (w.largest() > m) raise(w.largest());
-#pragma unroll
-      for (int e = 0; e < E; e += 2) sums.add(e / 2 % 2, w.get(e), w.get(e + 1), ExpSum::pack(-c0, -c0));
-      if (w.largest() >= bound) set_aside(w, c);
-    }
-  }
   for (int j = 0;; ++j) {
-    V next[kBatch];
     if (j + 1 < batches) load(next, j + 1);
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const float t = v[k].largest();
-      if (t >= bound) set_aside(v[k], lo + (j + k * batches) * kThreads + tid);
+      if (t >= bound) set_aside(v[k], v0 + (j + k * batches) * kThreads + tid);
       top = fmaxf(top, t);
     }
     if (top > m) raise(top);
@@ -299,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
       for (int e = 0; e < E; e += 2) sums.add(e / 2 % 2, v[k].get(e), v[k].get(e + 1), minus_c);
     if (j + 1 >= batches) break;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) v[k] = next[k];
+    for (int k = 0; k < kBatch; ++k) v[k] = vector(next[k]);
   }
   // the CTA's maximum and sum
   const float wm = warp_largest(m);
@@ -310,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.red[w]);
   const float held = fminf(fmaxf(m, -kHuge), kHuge), c1 = held * kLog2e;
   float part = sums.total() * exp2_fast(c0 - c1);
-  const int e0 = max(0, v0 * E - mis), e1 = min(p.V, v1 * E - mis);   // the slice's tokens
+  const int e0 = v0 * E, e1 = min(p.V, v1 * E);   // the slice's tokens
   if (held != m && isfinite(m)) {
     part = 0.f;
     for (int t = e0 + tid; t < e1; t += kThreads) {
@@ -346,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
       const float y = to_f(reinterpret_cast<const T*>(sh.vec)[f]);
       if (y >= bound) {
         const int at = next_place(&sh.keys);
-        if (at < kList) sh.list[at] = make_key(y, sh.at[f / E] * E - mis + f % E);
+        if (at < kList) sh.list[at] = make_key(y, sh.at[f / E] * E + f % E);
       }
     }
     __syncthreads();
@@ -449,9 +472,15 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 //
 // One CTA per request.  The n-th best of the slices' first candidates is a lower bound of the
 // result's n-th best.  What reaches it is gathered, and whoever has fewer than n better ones
-// writes itself to that place, so nothing depends on the order in which threads run.  With
-// more of them than the list holds (many equal scores) the ranks come from binary searches
-// in the sorted lists instead.
+// writes itself to that place, so nothing depends on the order in which threads run.  Where
+// few beams are far ahead that bound is loose, and the n-th best of 256 of those gathered
+// raises it first: 8 requests of 32 beams, 32 chosen, scores spread by 1: 23 us in all instead of 49.
+// With more of them than the list holds (many equal scores) the ranks come from binary
+// searches in the sorted lists instead.
+//
+// Bound: latency, of three dependent reads and the two ranks: 7 us behind the slices for 8
+// requests of 32 beams, 32 chosen (with 128-bit items instead of 64-bit scores and ties apart
+// 8; with one thread to an item instead of four 9).
 
 constexpr int kMergeList = 1024, kHeld = 8;
 constexpr int kTokenBits = 26;   // of the vocabulary (checked on the host)
@@ -496,7 +525,7 @@ template <int N> __device__ __forceinline__ float group_max(float x) {
   return x;
 }
 
-__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
+__global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
   __shared__ double lse[kMaxBeams], cum[kMaxBeams], bound;
   __shared__ float least[kMaxBeams];       // logits below are below the bound, by beam
   __shared__ unsigned long long head[kHeadItems];
@@ -562,46 +591,61 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
                 static_cast<unsigned>(tid);
   }
   __syncthreads();
-  // four threads count for one
-  for (int f = tid / 4; f < items; f += kMergeThreads / 4) {
-    const unsigned long long sc = head[f];
-    int rank = 0;
+  // bound = the n-th best of head's first `items`; four threads count for one
+  auto rank_head = [&](int items) {
+    for (int f = tid / 4; f < items; f += kMergeThreads / 4) {
+      const unsigned long long sc = head[f];
+      int rank = 0;
 #pragma unroll 4
-    for (int o = tid % 4; o < items; o += 4) rank += head[o] > sc;
-    rank = group_sum<4>(rank);
-    if (rank == p.n - 1) {
-      const double low = from_ordered(sc & ~255ull);
-      bound = isfinite(low) ? low : -INFINITY;
+      for (int o = tid % 4; o < items; o += 4) rank += head[o] > sc;
+      rank = group_sum<4>(rank);
+      if (rank == p.n - 1) {
+        const double low = from_ordered(sc & ~255ull);
+        bound = isfinite(low) ? low : -INFINITY;
+      }
     }
-  }
-  __syncthreads();
-  const double low = bound;
-  // below this logit no score reaches the bound: rounded down, far below what rounding the
-  // score in 64 bits can move; NaN for a beam without candidates, -inf without a bound
-  if (tid < p.K) {
-    const double x = low - cum[tid] + lse[tid];
-    least[tid] = !isfinite(lse[tid]) ? NAN
-                 : !isfinite(x)      ? -INFINITY
-                                     : static_cast<float>(x - 1e-6 * (1.0 + fabs(x)));
-  }
-  __syncthreads();
-  auto take = [&](int f, unsigned long long k) {
-    const int i = static_cast<int>(div_by(f, p.per_mul, p.per_shift));
-    if (k == 0 || !(key_logit(k) >= least[i])) return;
-    const double sc = score_of(i, k);
-    if (!(sc >= low)) return;
-    const int at = next_place(&count);
-    if (at < kMergeList) item[at] = make_item(sc, i, k);
+    __syncthreads();
   };
+  rank_head(items);
+  double low = bound;
+  for (;;) {
+    // below this logit no score reaches the bound: rounded down, far below what rounding the
+    // score in 64 bits can move; NaN for a beam without candidates, -inf without a bound
+    if (tid < p.K) {
+      const double x = low - cum[tid] + lse[tid];
+      least[tid] = !isfinite(lse[tid]) ? NAN
+                   : !isfinite(x)      ? -INFINITY
+                                       : static_cast<float>(x - 1e-6 * (1.0 + fabs(x)));
+    }
+    __syncthreads();
+    auto take = [&](int f, unsigned long long k) {
+      const int i = static_cast<int>(div_by(f, p.per_mul, p.per_shift));
+      if (k == 0 || !(key_logit(k) >= least[i])) return;
+      const double sc = score_of(i, k);
+      if (!(sc >= low)) return;
+      const int at = next_place(&count);
+      if (at < kMergeList) item[at] = make_item(sc, i, k);
+    };
 #pragma unroll
-  for (int u = 0; u < kHeld; ++u)
-    if (u * kMergeThreads + tid < total) take(u * kMergeThreads + tid, held[u]);
-  for (int f = kHeld * kMergeThreads + tid; f < total; f += kMergeThreads) take(f, all[f]);
-  if (tid < p.K && done[tid] && isfinite(cum[tid]) && cum[tid] >= low) {
-    const int at = next_place(&count);
-    if (at < kMergeList) item[at] = make_item(cum[tid], tid, 0);
+    for (int u = 0; u < kHeld; ++u)
+      if (u * kMergeThreads + tid < total) take(u * kMergeThreads + tid, held[u]);
+    for (int f = kHeld * kMergeThreads + tid; f < total; f += kMergeThreads) take(f, all[f]);
+    if (tid < p.K && done[tid] && isfinite(cum[tid]) && cum[tid] >= low) {
+      const int at = next_place(&count);
+      if (at < kMergeList) item[at] = make_item(cum[tid], tid, 0);
+    }
+    __syncthreads();
+    // Many where a few beams are far ahead of the others: the n-th best of some of them is a
+    // higher bound.
+    const int got = min(count, kMergeList), sample = min(got, kHeadItems);
+    if (got <= kHeadItems) break;
+    if (tid < sample) head[tid] = (item[tid * got / sample].hi & ~255ull) | static_cast<unsigned>(tid);
+    __syncthreads();
+    rank_head(sample);
+    if (!(bound > low)) break;   // equal ones, ranked below
+    if (tid == 0) count = 0;
+    low = bound;
   }
-  __syncthreads();
   // (rank, score, beam, token); with a bound there are n candidates at least
   auto place = [&](int rank, double sc, int i, int token) {
     const long long at = static_cast<long long>(b) * p.n + rank;
@@ -675,18 +719,26 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 // ------------------------------------------------------------------ host
 
 // Slices of a row of 16-byte vectors with `per` logits: more while the rows alone do not
-// give every SM two CTAs and a slice keeps a vector for each thread.
+// give every SM two CTAs and a slice keeps a vector for each thread, and on to twelve CTAs per
+// SM (three rounds of what is resident) while a slice keeps four batches.  64 x 8 rows of
+// 151936 bf16 logits: 4 / 5 / 7 slices 53 / 48 / 60 us.
 int slices_of(long long rows, int V, int per) {
-  const int vecs = V / per + 2;              // of an unaligned row
+  const int vecs = (V + per - 1) / per;
   int s = 1;
   while (rows * s < 2 * kSMs && vecs / (2 * s) >= kThreads) s *= 2;
-    while (rows * s < 12 * kSMs && vecs / (s + 1) >= 4 * kThreads * kBatch) ++s;
+  while (rows * s < 12 * kSMs && vecs / (s + 1) >= 4 * kThreads * kBatch) ++s;
   return s;
 }
 
 template <typename T>
 int launch(const BeamArgs& p, cudaStream_t st) {
-  beam_slice_kernel<T><<<dim3(p.B * p.K, p.slices), kThreads, 0, st>>>(p);
+  const dim3 grid(p.B * p.K, p.slices);
+  if (reinterpret_cast<uintptr_t>(p.logits) % 16 != 0 ||
+      (p.B > 1 && p.stride_batch * sizeof(T) % 16 != 0) ||
+      (p.K > 1 && p.stride_beam * sizeof(T) % 16 != 0))
+    beam_slice_kernel<T, true><<<grid, kThreads, 0, st>>>(p);
+  else
+    beam_slice_kernel<T, false><<<grid, kThreads, 0, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return GDN_ERR_LAUNCH;
   return launch_after(beam_merge_kernel, dim3(p.B), dim3(kMergeThreads), 0, st, p) == cudaSuccess
              ? GDN_OK : GDN_ERR_LAUNCH;
