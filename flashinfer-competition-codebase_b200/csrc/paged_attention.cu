@@ -233,11 +233,10 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   constexpr int MT = S::kTile / 16;                           // 16-token parts of a tile
   constexpr int kRows = 32 / CPR, kIters = S::kTile / kRows;  // rows a warp copies at a time
   constexpr uint32_t kAll = S::kTile == 32 ? 0xffffffffu : 0xffffu;
-  constexpr int kPad = kHeads * (D + 4) * 4 <= 2 * S::kHalf ? D + 4 : D;   // floats of a head in the merge
-  static_assert(kHeads * kPad * 4 <= 2 * S::kHalf, "the merge reuses a stage");
+  static_assert(kHeads * D * 4 <= 2 * S::kHalf, "the merge reuses a stage");
   static_assert(S::kStages == 3, "two tiles ahead of the one being multiplied");
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
+  __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads], sm_c[kHeads][kWarps];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
 
@@ -562,42 +561,87 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        const int d = i * 16 + lane / 4;
-        mine[h * kPad + d] = o[n][i][0];
-        mine[(h + 1) * kPad + d] = o[n][i][1];
-        mine[h * kPad + d + 8] = o[n][i][2];
-        mine[(h + 1) * kPad + d + 8] = o[n][i][3];
+        const int d = (i * 16 + lane / 4) ^ ((lane % 4) << 3);   // other heads, other banks
+        mine[h * D + d] = o[n][i][0];
+        mine[(h + 1) * D + d] = o[n][i][1];
+        mine[h * D + (d ^ 8)] = o[n][i][2];
+        mine[(h + 1) * D + (d ^ 8)] = o[n][i][3];
       }
     }
     __syncthreads();
     const int g = done.row / p.tiles, tile = done.row - g * p.tiles;
     const int head0 = g * p.group + tile * kHeads, heads = min(kHeads, p.group - tile * kHeads);
     const long long slot = 2 * static_cast<long long>(blockIdx.x) + (first_row ? 0 : 1);
-    for (int f0 = tid; f0 < heads * (D / 2); f0 += kWarps * 32) {
-      const int h = f0 / (D / 2), d = (f0 % (D / 2)) * 2;
-      float mx = sm_m[0][h];
+    const long long out0 = static_cast<long long>(done.b) * p.HQ + head0;
+    // the warps' factors for head h; `writes`: this thread writes the head's lse or m and l
+    auto factors = [&](int h, bool writes, float (&c)[kWarps]) {
+      float mx = sm_m[0][h], lt = 0.f;
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm_m[w][h]);
       const float base = mx == -INFINITY ? 0.f : mx;
-      float lt = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float c = exp2_fast(sm_m[w][h] - base);
-        const float* other =
-            reinterpret_cast<const float*>(smem + w * S::kWarpBytes + used * 2 * S::kHalf) + h * kPad + d;
-        lt += sm_l[w][h] * c;
-        a0 += other[0] * c;
-        a1 += other[1] * c;
+        c[w] = exp2_fast(sm_m[w][h] - base);
+        lt += sm_l[w][h] * c[w];
       }
       if (done.whole) {
-        const long long r = static_cast<long long>(done.b) * p.HQ + head0 + h;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        reinterpret_cast<uint32_t*>(p.out)[(r * D + d) / 2] = pack2<T>(a0 * inv, a1 * inv);
-        if (d == 0 && p.lse) p.lse[r] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
-      } else {
-        *reinterpret_cast<float2*>(p.part_o + (slot * kHeads + h) * D + d) = make_float2(a0, a1);
-        if (d == 0)
-          *reinterpret_cast<float2*>(p.part_ml + (slot * kHeads + h) * 2) = make_float2(mx, lt);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) c[w] *= inv;
+        if (writes && p.lse)
+          p.lse[out0 + h] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+      } else if (writes) {
+        *reinterpret_cast<float2*>(p.part_ml + (slot * kHeads + h) * 2) = make_float2(mx, lt);
+      }
+    };
+    // Four values a thread, several heads at once.  Where a thread has more than two heads
+    // the factors are computed once for all.
+    constexpr int kAtOnce = kWarps * 32 / (D / 4), kTurns = kHeads / kAtOnce;
+    constexpr int kUnroll = kTurns < 4 ? kTurns : 4;
+    constexpr bool kShared = kTurns > 2;
+    if constexpr (kShared) {
+      if (tid < kHeads) {
+        float c[kWarps];
+        factors(tid, tid < heads, c);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sm_c[tid][w] = c[w];
+      }
+      __syncthreads();
+    }
+    const int d = tid % (D / 4) * 4;
+#pragma unroll 1
+    for (int h0 = tid / (D / 4); h0 < heads; h0 += kUnroll * kAtOnce) {
+      float4 a[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int h = h0 + u * kAtOnce;
+        float c[kWarps];
+        if constexpr (kShared) {
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) c[w] = sm_c[h][w];
+        } else {
+          factors(h, d == 0 && h < heads, c);
+        }
+        a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(smem + w * S::kWarpBytes + used * 2 * S::kHalf +
+                                                            (h * D + (d ^ ((h & 6) << 2))) * 4);
+          a[u].x += x.x * c[w];
+          a[u].y += x.y * c[w];
+          a[u].z += x.z * c[w];
+          a[u].w += x.w * c[w];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int h = h0 + u * kAtOnce;
+        if (h >= heads) break;
+        if (done.whole)
+          reinterpret_cast<uint2*>(p.out)[((out0 + h) * D + d) / 4] =
+              make_uint2(pack2<T>(a[u].x, a[u].y), pack2<T>(a[u].z, a[u].w));
+        else
+          *reinterpret_cast<float4*>(p.part_o + (slot * kHeads + h) * D + d) = a[u];
       }
     }
     if (!more) break;
