@@ -71,7 +71,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& p, int n) {   // n: its 
 // no counters or flags have to be kept in memory.  In a call whose rows all are short
 // none is cut (cut == null): a row is then one unit of the line.
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;        // that take tiles of their own, alone or as teams
 
 // Shapes by head dim: tokens a warp takes at a time, ring stages, CTAs per SM.
 template <int D> struct Shape {
@@ -84,6 +84,11 @@ template <int D> struct Shape {
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kResident = D == 256 ? 1 : 2;
 };
+
+// Warps that share a tile, each with its own 8 of the row's heads: two where one warp's
+// registers do not hold 16 heads of 256 (100 sequences of 3000 tokens, 16 heads of 256 to a
+// key-value head: 60 us instead of 81).
+template <int D, int NG> constexpr int kTeam = D == 256 && NG == 2 ? 2 : 1;
 
 template <int kBlock> __device__ __forceinline__ int blocks_of(const AttnArgs& p, int b) {
   const int vis = sequence(p, p.lens[b]).vis;
@@ -105,9 +110,9 @@ struct Share {
 };
 
 // This CTA's share, by all its threads; start == end where there is none.
-template <int kBlock> __device__ Share my_share(const AttnArgs& p) {
-  constexpr int N = kWarps * 32;
-  __shared__ long long sum[kWarps], found_before;
+template <int kBlock, int kCtaWarps> __device__ Share my_share(const AttnArgs& p) {
+  constexpr int N = kCtaWarps * 32;
+  __shared__ long long sum[kCtaWarps], found_before;
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, rows = p.HKV * p.tiles;
   long long base = 0, first = 0;
@@ -136,7 +141,7 @@ template <int kBlock> __device__ Share my_share(const AttnArgs& p) {
     __syncthreads();
     first = base + x - n;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kCtaWarps; ++w) {
       first += w < warp ? sum[w] : 0;
       base += sum[w];
     }
@@ -226,22 +231,25 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // along a row is one XOR on the address.
 
 template <typename T, int D, int NG>
-__global__ void __launch_bounds__(kWarps * 32, Shape<D>::kResident)
+__global__ void __launch_bounds__(kWarps * kTeam<D, NG> * 32, Shape<D>::kResident)
 attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   using S = Shape<D>;
   constexpr int kHeads = 8 * NG, KS = D / 16, CPR = D / 8;    // chunks per row
+  constexpr int kMates = kTeam<D, NG>, G = NG / kMates;       // groups of 8 heads of one warp
+  constexpr int kThreads = kWarps * kMates * 32;
   constexpr int MT = S::kTile / 16;                           // 16-token parts of a tile
-  constexpr int kRows = 32 / CPR, kIters = S::kTile / kRows;  // rows a warp copies at a time
+  constexpr int kRows = 32 / CPR * kMates;                    // rows a team copies at a time
+  constexpr int kIters = S::kTile / kRows;
   constexpr uint32_t kAll = S::kTile == 32 ? 0xffffffffu : 0xffffu;
   static_assert(kHeads * D * 4 <= 2 * S::kHalf, "the merge reuses a stage");
   static_assert(S::kStages == 3, "two tiles ahead of the one being multiplied");
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads], sm_c[kHeads][kWarps];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = tid / 32 / kMates, mate = tid / 32 % kMates, lane = tid % 32;
   const uint32_t ring = smem_addr(smem) + warp * S::kWarpBytes;
 
   grid_trigger();                         // the join's CTAs may take their places and wait
-  const Share share = my_share<S::kBlock>(p);
+  const Share share = my_share<S::kBlock, kWarps * kMates>(p);
   const int rows = p.HKV * p.tiles;                           // rows of one sequence
   long long at = share.start, before = share.before;
   if (at == share.end) {
@@ -249,8 +257,13 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     return;
   }
 
+  auto team_sync = [&]() {
+    if constexpr (kMates == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp), "n"(kMates * 32) : "memory");
+  };
+
   // fixed parts of this lane's addresses
-  const int copy_r = lane / CPR, copy_c = lane % CPR;
+  const int copy_r = mate * (32 / CPR) + lane / CPR, copy_c = lane % CPR;
   const uint32_t copy_at = copy_r * S::kRow + ((copy_c ^ copy_r) << 4);
   const uint32_t k_at = (lane % 16) * S::kRow + (((lane >> 4) ^ (lane & 7)) << 4);
   const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * S::kRow + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
@@ -335,7 +348,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     const int off = tok < 0 ? 0 : tok - static_cast<int>(div_by(tok, p.page_mul, p.page_shift)) * p.page_size;
     const bool is_new = f.append && tok == f.len - 1;
     const bool in_cache = tok >= 0 && page >= 0 && page < p.num_pages;
-    if (f_row == 0 && p.bad != nullptr && lane < S::kTile && tok >= 0 && page >= p.num_pages &&
+    if (f_row == 0 && p.bad != nullptr && mate == 0 && lane < S::kTile && tok >= 0 && page >= p.num_pages &&
         first_in_page(tok, off))
       atomicAdd(p.bad, 1);
     const uint32_t seen = __ballot_sync(0xffffffffu, in_cache || is_new) & kAll;
@@ -389,13 +402,13 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     }
   };
   // queries as the right operand: head lane / 4 (+ 8 per further group), two dims a register
-  uint32_t qf[NG][KS][2];
+  uint32_t qf[G][KS][2];
   auto load_queries = [&]() {
     const int g = row.row / p.tiles, tile = row.row - g * p.tiles;
     const int heads = min(kHeads, p.group - tile * kHeads);
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      const int h = n * 8 + lane / 4;
+    for (int n = 0; n < G; ++n) {
+      const int h = (mate * G + n) * 8 + lane / 4;
       const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q) +
                           (static_cast<long long>(row.b) * p.HQ + g * p.group + tile * kHeads +
                            (h < heads ? h : 0)) * (D / 2);
@@ -427,10 +440,10 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   fetch();
   advance();
 
-  float o[NG][KS][4], m[NG][2], l[NG][2];
+  float o[G][KS][4], m[G][2], l[G][2];
   auto clear = [&]() {
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
+    for (int n = 0; n < G; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
@@ -445,15 +458,15 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
   while (true) {
     if (ahead == 2) copy_wait<1>();
     else copy_wait<0>();
-    __syncwarp();
+    team_sync();
     const uint32_t buf = ring + st * 2 * S::kHalf;
     const uint32_t seen = mask[0];
-    float y[MT][NG][4];
+    float y[MT][G][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float x[NG][2][4];                  // two chains of products
+      float x[G][2][4];                  // two chains of products
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < G; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[n][0][j] = x[n][1][j] = 0.f;
 #pragma unroll
@@ -461,10 +474,10 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
         uint32_t a[4];
         load_matrices(a, (buf + k_at + t * 16 * S::kRow) ^ (i * 32));
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
+        for (int n = 0; n < G; ++n) mma<T>(x[n][i & 1], a, qf[n][i][0], qf[n][i][1]);
       }
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < G; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[t][n][j] = (x[n][0][j] + x[n][1][j]) * p.scale_log2;
     }
@@ -472,14 +485,14 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
+        for (int n = 0; n < G; ++n) {
           if (!((seen >> (t * 16 + lane / 4)) & 1)) y[t][n][0] = y[t][n][1] = -INFINITY;
           if (!((seen >> (t * 16 + lane / 4 + 8)) & 1)) y[t][n][2] = y[t][n][3] = -INFINITY;
         }
     }
-    uint32_t pb[MT][NG][2];
+    uint32_t pb[MT][G][2];
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
+    for (int n = 0; n < G; ++n) {
       float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -524,9 +537,9 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
         uint32_t a[4];
         load_matrices_t(a, (buf + S::kHalf + v_at + t * 16 * S::kRow) ^ (i * 32));
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mma<T>(o[n][i], a, pb[t][n][0], pb[t][n][1]);
+        for (int n = 0; n < G; ++n) mma<T>(o[n][i], a, pb[t][n][0], pb[t][n][1]);
       }
-    __syncwarp();                         // every lane is done with this stage
+    team_sync();                          // every lane is done with this stage
     --ahead;
     mask[0] = mask[1];
     fetch();
@@ -546,13 +559,13 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     }
     float* mine = reinterpret_cast<float*>(smem + warp * S::kWarpBytes + used * 2 * S::kHalf);
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
+    for (int n = 0; n < G; ++n) {
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], d);
         l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], d);
       }
-      const int h = n * 8 + 2 * (lane % 4);
+      const int h = (mate * G + n) * 8 + 2 * (lane % 4);
       if (lane < 4) {
         sm_m[warp][h] = m[n][0];
         sm_m[warp][h + 1] = m[n][1];
@@ -596,7 +609,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
     };
     // Four values a thread, several heads at once.  Where a thread has more than two heads
     // the factors are computed once for all.
-    constexpr int kAtOnce = kWarps * 32 / (D / 4), kTurns = kHeads / kAtOnce;
+    constexpr int kAtOnce = kThreads / (D / 4), kTurns = kHeads / kAtOnce;
     constexpr int kUnroll = kTurns < 4 ? kTurns : 4;
     constexpr bool kShared = kTurns > 2;
     if constexpr (kShared) {
@@ -758,7 +771,7 @@ template <typename T, int D, int NG>
 cudaError_t launch_shape(const AttnArgs& p, const Plan& q, cudaStream_t st) {
   cudaError_t e = allow_smem<attn_decode_kernel<T, D, NG>>(Shape<D>::kSmem);
   if (e != cudaSuccess) return e;
-  attn_decode_kernel<T, D, NG><<<p.grid, kWarps * 32, Shape<D>::kSmem, st>>>(p);
+  attn_decode_kernel<T, D, NG><<<p.grid, kWarps * kTeam<D, NG> * 32, Shape<D>::kSmem, st>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess || !q.split) return e;
   const unsigned x = static_cast<unsigned>(q.cut);
