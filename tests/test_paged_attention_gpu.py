@@ -163,6 +163,17 @@ def test_bad_pages_are_counted_once_with_a_window(sinks, window):
     assert int(bad) == want[-1]
 
 
+@pytest.mark.parametrize("HQ,HKV", [(12, 1), (40, 2)])
+@pytest.mark.parametrize("lens", [[100, 30, 90], [1500], [5] * 200])
+def test_bad_pages_with_two_warps_to_a_tile(HQ, HKV, lens):
+    x = make(lens, HQ, HKV, 256, 16)
+    x["block_tables"][:, 1::3] = 99999
+    want = expect(x)
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(x, run(x, bad_index_count=bad), want)
+    assert int(bad) == want[-1]
+
+
 def test_lengths_beyond_the_table_and_negative():
     x = make([40, -3, 10], 8, 2, 128, 16, width=3)
     x["seq_lens"][0] = 49
