@@ -43,6 +43,9 @@ struct Pools {
 // touches that column, so sources that are destinations too (a permutation of beams, a
 // cycle) are read before they are overwritten, without a second buffer; a source with several
 // destinations is read from HBM once, since its readers are in one CTA.
+//
+// Bound: HBM.  256 pairs of 2 MB, 161 of the sources different: 157 us (875 MB, 5.6 TB/s; a
+// plain copy, which writes as much as it reads, 6.57).  4 pairs of 512 KB: 3.5 us, latency.
 
 struct CopyArgs {
   Pools pools;
@@ -176,6 +179,10 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
 //
 // Pairs whose destinations are no other pair's source (fork, compact): a work item is a
 // segment of one pair's page, and any CTA may take it at any time.
+//
+// Bound: HBM for compaction (8191 pages of 32 KB in two pools, half of them live: 48 us with its
+// plan, 269 MB, 5.6 TB/s); for forks the latency of three launches of which two overlap (512
+// rows, up to 4000 tokens: 14.5 us, 22 MB).
 
 struct MoveArgs {
   Pools pools;

@@ -225,7 +225,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // buffers in shared memory with asynchronous copies, so the main loop has no CTA barrier.
 // A tile's page numbers are loaded one tile before its copies are issued, and the copies run
 // on into the share's next row, so a short row does not empty the pipeline.
-
+//
+// Bound: HBM; a cached byte takes part in one operation for each head of its group, far below
+// the tensor cores' rate, so the warp-level instructions, whose operands need no staging
+// through tensor memory, are enough.  64 sequences of 820 to 8191 tokens, 32 heads over 8 of 128: 242 us
+// (1.59 GB, 6.56 TB/s, all of a copy's rate).  One of 131072 tokens, 16 heads over 2 of 256: 52 us
+// (268 MB, 5.1 TB/s): 46 and the join, whose latency nothing hides.  One of 100 tokens: 5.3 us,
+// the latency of a launch and five dependent reads.
+//
 // A tile's row r has its 16-byte chunk c at r kRow + ((c ^ (r & 7)) << 4): the eight rows that a
 // matrix load touches lie in different banks.  Stages are aligned to rows, so stepping
 // along a row is one XOR on the address.
@@ -670,7 +677,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 // CTA (x, y): kValues values from y kValues of the row of cut[x].  kValues / 4 threads take
 // four values each; the CTA's groups of them take every kGroups-th part.  Few rows have many
 // parts each: then a CTA takes few values and has many groups (131072 tokens in 148 parts:
-// 56 us with 512 values and 2 groups, 51 us with 128 and 8).
+// 57 us with 512 values and 2 groups, 52 us with 128 and 8).
 constexpr int kJoinThreads = 256, kJoinParts = 2 * kSMs;
 
 template <typename T, int D, int NG, int kValues>
@@ -741,10 +748,11 @@ int heads_of(int group) { return group <= 8 ? 8 : 16; }
 int block_of(int D) { return D == 64 ? Shape<64>::kBlock : D == 128 ? Shape<128>::kBlock : Shape<256>::kBlock; }
 int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
 
-// Rows are not cut where that leaves no CTA more than about 2.5 blocks over an even share:
-// less than the cut's partial sums and the join cost.  Not cut / cut: 1 row of 100 tokens of
-// 128 dims 5.8 / 7.1 us, of 512 tokens 10.7 / 7.1 us; 512 rows of 256 tokens 14.8 / 22.1 us,
-// of 500 tokens 22.4 / 30.5 us.
+// Rows are not cut where that leaves no CTA more than about 4 blocks over an even share: less
+// than the cut's partial sums and the join cost.  Not cut / cut: 1 row of 100 tokens of 128 dims
+// 5.3 / 7.0 us, of 512 tokens 10.2 / 7.1 us; 512 rows of 256 tokens 14.4 / 18.0 us, of 500
+// tokens 27.8 / 30.0 us; 300 rows of 330 tokens of 64 dims 12.3 / 14.8 us; of 256 dims 75 rows 11.5
+// / 15.0 us, 150 rows 20.2 / 19.0 us.
 
 struct Plan {
   long long rows, grid;      // rows of a call; CTAs: what the GPU holds at once, or fewer
@@ -759,7 +767,7 @@ Plan plan_of(int B, int HQ, int HKV, int D, long long max_tokens) {
   const long long nb = max_tokens > 0 ? (max_tokens + block_of(D) - 1) / block_of(D) : 1;
   const long long most = static_cast<long long>(kSMs) * resident(D);
   const long long waves = (q.rows + most - 1) / most;
-  q.split = 2 * nb * (waves * most - q.rows) > 5 * most;
+  q.split = nb * (waves * most - q.rows) > 4 * most;
   const long long units = q.rows * (q.split ? nb : 1);
   q.grid = units < most ? units : most;
   q.cut = static_cast<size_t>(q.rows <= q.grid ? q.rows : q.grid);
