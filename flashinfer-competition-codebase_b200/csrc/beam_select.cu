@@ -96,7 +96,7 @@ template <typename T> struct Vec {
 //
 // A row's slices are counted in vectors of 16 bytes from its first token, and a row that need
 // not begin on a 16-byte boundary is read in words of 32 bits (64 x 8 rows of 151936 bf16
-// logits: 55 us instead of 49): equal rows get equal sums, bit for bit, wherever they lie, so
+// logits: 51 us instead of 46): equal rows get equal sums, bit for bit, wherever they lie, so
 // that equal beams tie.
 //
 // One pass over the slice.  Every thread keeps its own running maximum and its sum of
@@ -351,9 +351,10 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     if (held == m) s *= static_cast<double>(exp2f(-fmaf(held, kLog2e, -c1)));   // what c's rounding took
     p.sums[static_cast<long long>(row) * p.slices + slice] = make_float2(m, static_cast<float>(s));
   }
-  // a sharper bound from up to 256 of the vectors set aside, as before: whole warps of them
+  // a sharper bound from up to 256 of the vectors set aside, as before: whole warps of them,
+  // where there is more to rank than a candidate a thread
   const int aside = min(sh.count, kList), wide = min(aside, kThreads) / 32;
-  const int nth = wide > 0 ? (p.n + wide - 1) / wide : 33;
+  const int nth = aside * E > kThreads && wide > 0 ? (p.n + wide - 1) / wide : 33;
   if (warp < wide && nth <= 32) {
     const float y = warp_nth(V{sh.vec[tid]}.largest(), nth);
     if (lane == 0) sh.red[warp] = y;
@@ -470,15 +471,16 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
 
 // ------------------------------------------------------------------ the merge
 //
-// One CTA per request.  The n-th best of the slices' first candidates is a lower bound of the
-// result's n-th best.  What reaches it is gathered, and whoever has fewer than n better ones
+// One CTA per request.  The n-th best of the first candidates of live beams' slices, 4 n of them, is a
+// lower bound of the result's n-th best (64 x 8 beams of 151936, 16 chosen: with 1 / 2 / 4 / 8 n
+// 49.2 / 49.3 / 45.6 / 46.5 us).  What reaches it is gathered, and whoever has fewer than n better ones
 // writes itself to that place, so nothing depends on the order in which threads run.  Where
 // few beams are far ahead that bound is loose, and the n-th best of 256 of those gathered
-// raises it first: 8 requests of 32 beams, 32 chosen, scores spread by 1: 23 us in all instead of 49.
+// raises it first: 8 requests of 32 beams, 32 chosen, scores spread by 1: 22 us in all instead of 49.
 // With more of them than the list holds (many equal scores) the ranks come from binary
 // searches in the sorted lists instead.
 //
-// Bound: latency, of three dependent reads and the two ranks: 7 us behind the slices for 8
+// Bound: latency, of three dependent reads and the two ranks: 6 us behind the slices for 8
 // requests of 32 beams, 32 chosen (with 128-bit items instead of 64-bit scores and ties apart
 // 8; with one thread to an item instead of four 9).
 
@@ -532,6 +534,7 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
   __shared__ MergeItem item[kMergeList];
   __shared__ int count;
   __shared__ bool done[kMaxBeams];
+  __shared__ int live_beam[kMaxBeams], live;   // beams with candidates of their own
   const int b = blockIdx.x, tid = threadIdx.x;
   const int per_beam = p.slices * p.n, lists = p.K * p.slices, total = lists * p.n;
   if (tid == 0) {
@@ -544,10 +547,21 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
     done[tid] = p.finished && p.finished[b * p.K + tid];
   }
   __syncthreads();
+  if (tid < 32) {
+    int before = 0;
+    for (int i = tid; i - tid < p.K; i += 32) {
+      const bool on = i < p.K && !done[i] && isfinite(cum[i]);
+      const uint32_t all_on = __ballot_sync(0xffffffffu, on);
+      if (on) live_beam[before + __popc(all_on & ((1u << tid) - 1))] = i;
+      before += __popc(all_on);
+    }
+    if (tid == 0) live = before;
+  }
+  __syncthreads();
   grid_wait();
-  // everything that is read comes at once: up to kHeld keys a thread, the first candidates
-  // (the first `depth` of every slice, of as many slices as fit; at least n where there are
-  // as many), and the slices' sums, eight threads to a beam
+  // everything that is read comes at once: up to kHeld keys a thread, the first `depth`
+  // candidates of every live beam's slices (of as many as fit), and the slices' sums, eight
+  // threads to a beam
   const unsigned long long* all = p.keys + static_cast<long long>(b) * total;
   unsigned long long held[kHeld];
 #pragma unroll
@@ -555,8 +569,16 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
     const int f = u * kMergeThreads + tid;
     held[u] = f < total ? all[f] : 0;
   }
-  const int depth = (p.n + lists - 1) / lists, items = min(lists * depth, kHeadItems);
-  const unsigned long long head_key = tid < items ? all[tid % lists * p.n + tid / lists] : 0;
+  const int live_lists = live * p.slices;
+  const int depth = live ? min(p.n, (4 * p.n + live_lists - 1) / live_lists) : 0;
+  const int items = min(live_lists * depth, kHeadItems);
+  unsigned long long head_key = 0;
+  int head_beam = 0;
+  if (tid < items) {
+    const int l = tid % live_lists, i = l / p.slices;
+    head_beam = live_beam[i];
+    head_key = all[(head_beam * p.slices + l - i * p.slices) * p.n + tid / live_lists];
+  }
   const int i8 = tid / 8, s8 = tid % 8;
   if (i8 < p.K) {
     double l = NAN;                     // not finite: a beam without candidates of its own
@@ -583,11 +605,9 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
   auto score_of = [&](int i, unsigned long long k) {
     return cum[i] + (static_cast<double>(key_logit(k)) - lse[i]);
   };
-  // a slice that wrote nothing (its beam is finished or dead) leaves stale keys: lse says so
   if (tid < items) {
-    const int i = tid % lists / p.slices;
     // all different: the last 8 bits are the place instead of the score's, which rounds down
-    head[tid] = (ordered(head_key && isfinite(lse[i]) ? score_of(i, head_key) : -INFINITY) & ~255ull) |
+    head[tid] = (ordered(head_key && isfinite(lse[head_beam]) ? score_of(head_beam, head_key) : -INFINITY) & ~255ull) |
                 static_cast<unsigned>(tid);
   }
   __syncthreads();
@@ -606,7 +626,7 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
     }
     __syncthreads();
   };
-  rank_head(items);
+  if (items >= p.n) rank_head(items);
   double low = bound;
   for (;;) {
     // below this logit no score reaches the bound: rounded down, far below what rounding the
@@ -720,8 +740,9 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
 
 // Slices of a row of 16-byte vectors with `per` logits: more while the rows alone do not
 // give every SM two CTAs and a slice keeps a vector for each thread, and on to twelve CTAs per
-// SM (three rounds of what is resident) while a slice keeps four batches.  64 x 8 rows of
-// 151936 bf16 logits: 4 / 5 / 7 slices 53 / 48 / 60 us.
+// SM (three rounds of what is resident) while a slice keeps four batches.  All of 64 x 8 rows of
+// 151936 bf16 logits, 2 / 3 / 4 / 5 / 7 slices: 65 / 49 / 49 / 51 / 57 us; 55 x 10 rows of 80000,
+// 1 / 2 / 3: 31.0 / 31.4 / 35.8 us; 18 x 10 rows of 151936, 2 / 3 / 4: 41 / 26 / 26 us.
 int slices_of(long long rows, int V, int per) {
   const int vecs = (V + per - 1) / per;
   int s = 1;
