@@ -23,6 +23,10 @@ using namespace gdn_serving;
 constexpr int kMaxBeams = 64, kMaxSelected = 64;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBatch = 4;        // 16-byte vectors of logits a thread takes at a time
+constexpr int kTop = 32 / kWarps;  // lane maxima of each warp, up to kSharp-th largest of all of them
+// is a bound; for larger n the warps' own ones are about as sharp, and cheaper.  The one / the other:
+// 18 x 10 rows of 151936 logits, n = 20: 23.8 / 26.1 us; 8 x 12 of 116858, n = 24: 18.1 / 17.5 us.
+constexpr int kSharp = 20;
 constexpr int kList = 1024;      // vectors, then candidates, that a slice gathers
 constexpr int kMergeThreads = 512;
 constexpr int kHeadItems = 256;  // of the merge's bound, at most 256
@@ -96,22 +100,24 @@ template <typename T> struct Vec {
 //
 // A row's slices are counted in vectors of 16 bytes from its first token, and a row that need
 // not begin on a 16-byte boundary is read in words of 32 bits (64 x 8 rows of 151936 bf16
-// logits: 51 us instead of 46): equal rows get equal sums, bit for bit, wherever they lie, so
+// logits: 47 us instead of 42): equal rows get equal sums, bit for bit, wherever they lie, so
 // that equal beams tie.
 //
 // One pass over the slice.  Every thread keeps its own running maximum and its sum of
 // exponentials relative to it, so the loop has no barrier; its next batch of vectors is in
-// flight while it works on one.  The first batch is a sample spread over the slice: with
-// r = ceil(n / warps), the smallest of the warps' r-th largest lane maxima, T, has n logits
-// at or above it.  Vectors that reach T are set aside as they are; at the end the n-th
-// largest of their maxima is a sharper bound, and what reaches that is ranked.
+// flight while it works on one.  The first batch is a sample spread over the slice, which gives a
+// bound T that n logits reach: the n-th largest of the warps' four largest lane maxima, or
+// for larger n the smallest of the warps' ceil(n / warps)-th largest.  Vectors that reach T are set
+// aside as they are; at the end the n-th largest of their maxima is a sharper bound, and what
+// reaches that is ranked.  Raising T on the way takes barriers, which cost more than it saves
+// (64 x 8 rows of 151936 logits: 47 us with, 43 without).
 //
 // Bound: the issue of instructions.  The exponentials alone come near HBM for 16-bit logits
 // (12.3 logits a clock and SM at the measured copy rate, of 16 exponentials), so an element
 // costs one unpack, one exponential, half of a packed multiply-add and of a packed addition,
 // and parts of packed maxima: 94 instructions for a vector of eight with all that is set
-// aside.  64 x 8 rows of 151936 bf16 logits, a tenth finished: 42 us (140 MB, 3.3 TB/s, 28.7
-// million warp instructions; a copy's rate would read them in 21).  8 x 32 rows of 50257 fp32, a
+// aside.  64 x 8 rows of 151936 bf16 logits, a tenth finished: 39 us (140 MB, 3.6 TB/s; a copy's
+// rate would read them in 21).  8 x 32 rows of 50257 fp32, a
 // quarter finished: 15 us (39 MB, 2.6 TB/s; 14 with rows padded to begin on 16 bytes).
 // Tried there without gain: three to eight CTAs an SM (41 to 72 us), batches of 2 and 8, a ring
 // of asynchronous copies through shared memory (50), places by ballots (55).
@@ -121,6 +127,7 @@ struct SliceShared {
   int at[kList];                   // their places in the row
   unsigned long long list[kList];  // keys of candidates
   float red[kWarps];
+  alignas(16) float top[32];
   float sum[kWarps];
   int scan[kWarps];
   unsigned long long best[kWarps];
@@ -279,14 +286,32 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   for (int k = 0; k < kBatch; ++k) v[k] = vector(next[k]);
 #pragma unroll
   for (int k = 0; k < kBatch; ++k) m = fmaxf(m, v[k].largest());
-  {
+  float bound;
+  if (p.n <= kSharp) {
+    // the n-th largest of the warps' kTop largest lane maxima
+    float x = m, mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kTop; ++i) {
+      const float y = warp_largest(x);
+      if (lane == i) mine = y;
+      const uint32_t same = __ballot_sync(0xffffffffu, x == y);
+      if (same && lane == __ffs(same) - 1) x = -INFINITY;
+    }
+    if (lane < kTop) sh.top[warp * kTop + lane] = fmaxf(mine, -FLT_MAX);
+    __syncthreads();
+    const float y = sh.top[lane];
+    int reach = 0;               // of the 32 are at least y
+#pragma unroll
+    for (int i = 0; i < 32; ++i) reach += sh.top[i] >= y;
+    bound = warp_largest(reach >= p.n ? y : -INFINITY);
+  } else {
     const float nth = warp_nth(m, (p.n + kWarps - 1) / kWarps);
     if (lane == 0) sh.red[warp] = nth;
-  }
-  __syncthreads();
-  float bound = sh.red[0];
+    __syncthreads();
+    bound = sh.red[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.red[w]);
+    for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.red[w]);
+  }
   unsigned long long* out = p.keys + (static_cast<long long>(row) * p.slices + slice) * p.n;
   // s = sum of 2^(x log2 e - c), c = m log2 e as rounded (within +-kHuge), in four chains
   float c0 = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
@@ -739,15 +764,18 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
 // ------------------------------------------------------------------ host
 
 // Slices of a row of 16-byte vectors with `per` logits: more while the rows alone do not
-// give every SM two CTAs and a slice keeps a vector for each thread, and on to twelve CTAs per
-// SM (three rounds of what is resident) while a slice keeps four batches.  All of 64 x 8 rows of
-// 151936 bf16 logits, 2 / 3 / 4 / 5 / 7 slices: 65 / 49 / 49 / 51 / 57 us; 55 x 10 rows of 80000,
-// 1 / 2 / 3: 31.0 / 31.4 / 35.8 us; 18 x 10 rows of 151936, 2 / 3 / 4: 41 / 26 / 26 us.
-int slices_of(long long rows, int V, int per) {
-  const int vecs = (V + per - 1) / per;
+// give every SM two CTAs and a slice keeps a vector for each thread, on to 500 CTAs (of 592
+// that are resident) while a slice keeps four batches, and on to twelve an SM while it keeps 65536 logits,
+// or for n > 16 four batches: a longer slice sets more aside.  1 / 2 / 3 / 4 slices, n = 16: 64 x 8 rows of
+// 151936 bf16 logits 45 / 43 / 47 / 48 us, 55 x 10 of 80000 28 / 30 / 36 / 39, 18 x 10 of 151936 31 / 25
+// / 24 / 24, 64 x 8 of 100352 fp32 41 / 44 / 46 / 49; n = 64: 8 x 32 of 100352 bf16 92 / 53 / 42 / 46.
+int slices_of(long long rows, int V, int per, int n) {
+  const int vecs = (V + per - 1) / per, batches = 4 * kThreads * kBatch;
+  const int enough = n <= 16 ? 65536 / per : batches;
   int s = 1;
   while (rows * s < 2 * kSMs && vecs / (2 * s) >= kThreads) s *= 2;
-  while (rows * s < 12 * kSMs && vecs / (s + 1) >= 4 * kThreads * kBatch) ++s;
+  while (rows * s < 500 && vecs / (s + 1) >= batches) ++s;
+  while (rows * s < 12 * kSMs && vecs / (s + 1) >= enough) ++s;
   return s;
 }
 
@@ -772,7 +800,7 @@ extern "C" {
 size_t gdn_beam_select_workspace_bytes(int B, int K, int V, int n) {
   if (B < 1 || K < 1 || V < 1 || n < 1) return 0;
   const long long rows = static_cast<long long>(B) * K;
-  return static_cast<size_t>(rows) * std::max(slices_of(rows, V, 4), slices_of(rows, V, 8)) * (static_cast<size_t>(n) * 8 + 8);
+  return static_cast<size_t>(rows) * std::max(slices_of(rows, V, 4, n), slices_of(rows, V, 8, n)) * (static_cast<size_t>(n) * 8 + 8);
 }
 
 int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch, int64_t stride_beam,
@@ -795,7 +823,7 @@ int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch, int64_t
   BeamArgs p{};
   p.logits = logits; p.scores = scores; p.finished = finished; p.tokens = tokens;
   p.parents = parents; p.out_scores = new_scores;
-  p.slices = slices_of(static_cast<long long>(B) * K, V, dtype == GDN_DTYPE_FP32 ? 4 : 8);
+  p.slices = slices_of(static_cast<long long>(B) * K, V, dtype == GDN_DTYPE_FP32 ? 4 : 8, n);
   p.keys = static_cast<unsigned long long*>(workspace);
   p.sums = reinterpret_cast<float2*>(p.keys + static_cast<size_t>(B) * K * p.slices * n);
   p.stride_batch = stride_batch; p.stride_beam = stride_beam;
