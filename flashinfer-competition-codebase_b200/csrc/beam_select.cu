@@ -127,7 +127,7 @@ struct SliceShared {
   int at[kList];                   // their places in the row
   unsigned long long list[kList];  // keys of candidates
   float red[kWarps];
-  alignas(16) float top[32];
+  float top[32];                   // its own place: red is written again without a barrier between
   float sum[kWarps];
   int scan[kWarps];
   unsigned long long best[kWarps];
@@ -306,11 +306,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     bound = warp_largest(reach >= p.n ? y : -INFINITY);
   } else {
     const float nth = warp_nth(m, (p.n + kWarps - 1) / kWarps);
-    if (lane == 0) sh.red[warp] = nth;
+    if (lane == 0) sh.top[warp] = nth;
     __syncthreads();
-    bound = sh.red[0];
+    bound = sh.top[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.red[w]);
+    for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.top[w]);
   }
   unsigned long long* out = p.keys + (static_cast<long long>(row) * p.slices + slice) * p.n;
   // s = sum of 2^(x log2 e - c), c = m log2 e as rounded (within +-kHuge), in four chains
