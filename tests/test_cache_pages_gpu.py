@@ -197,6 +197,26 @@ def test_compact(P, live):
         assert torch.equal(p.cpu(), w)
 
 
+@pytest.mark.parametrize("P", [5, 4096, 16385, 40003])
+def test_counts_that_do_not_begin_on_16_bytes(P):
+    g = torch.Generator().manual_seed(P)
+    ref = torch.randint(-1, 3, (P,), generator=g, dtype=I32)
+    for off in (1, 2, 3):
+        r = torch.full((P + 8,), 7, dtype=I32, device="cuda")
+        r[off:off + P] = ref.cuda()
+        want = serving_ref.compact(ref, None, [])
+        remap, n = gdn_b200.compact_pages(r[off:off + P])
+        assert torch.equal(remap.cpu(), want[0]) and int(n) == want[1]
+        assert torch.equal(r[off:off + P].cpu(), want[2])
+        assert r[:off].eq(7).all() and r[off + P:].eq(7).all()
+        r[off:off + P] = ref.cuda()
+        free = (ref <= 0).nonzero()[:, 0].tolist()
+        need = torch.ones(len(free) + 3, dtype=torch.bool, device="cuda")
+        pages = gdn_b200.alloc_pages(r[off:off + P], need)
+        assert pages.tolist() == free + [-1] * 3
+        assert r[off:off + P].gt(0).all() and r[:off].eq(7).all() and r[off + P:].eq(7).all()
+
+
 def test_compact_without_tables_or_pools():
     r = ints([0, 2, 0, 1])
     remap, n = gdn_b200.compact_pages(r)
