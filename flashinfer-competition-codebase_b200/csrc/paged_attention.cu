@@ -229,8 +229,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // Bound: HBM; a cached byte takes part in one operation for each head of its group, far below
 // the tensor cores' rate, so the warp-level instructions, whose operands need no staging
 // through tensor memory, are enough.  64 sequences of 820 to 8191 tokens, 32 heads over 8 of 128: 242 us
-// (1.59 GB, 6.56 TB/s, all of a copy's rate).  One of 131072 tokens, 16 heads over 2 of 256: 52 us
-// (268 MB, 5.1 TB/s): 46 and the join, whose latency nothing hides.  One of 100 tokens: 5.3 us,
+// (1.59 GB, 6.56 TB/s, all of a copy's rate).  One of 131072 tokens, 16 heads over 2 of 256: 51 us
+// (268 MB, 5.2 TB/s): 46 and the join, whose latency nothing hides.  One of 100 tokens: 5.3 us,
 // the latency of a launch and five dependent reads.
 //
 // A tile's row r has its 16-byte chunk c at r kRow + ((c ^ (r & 7)) << 4): the eight rows that a
@@ -676,8 +676,9 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 // Adds up the parts of the rows that were cut: o = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
 // CTA (x, y): kValues values from y kValues of the row of cut[x].  kValues / 4 threads take
 // four values each; the CTA's groups of them take every kGroups-th part.  Few rows have many
-// parts each: then a CTA takes few values and has many groups (131072 tokens in 148 parts:
-// 57 us with 512 values and 2 groups, 52 us with 128 and 8).
+// parts each: then a CTA takes few values and has many groups.  131072 tokens, 16 heads of 128 to
+// one key-value head, 296 parts: 20.5 us in all with 32 values, 21.9 with 64, 23.5 with 128; but
+// 4 x 16000 tokens, 64 heads over 4 of 256, where 32 values make 2048 CTAs: 54 us, 51 with 128.
 constexpr int kJoinThreads = 256, kJoinParts = 2 * kSMs;
 
 template <typename T, int D, int NG, int kValues>
@@ -686,7 +687,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   constexpr int kQuads = kValues / 4, kGroups = kJoinThreads / kQuads;
   __shared__ float2 ml[kJoinParts][kHere];
   __shared__ float4 acc[kGroups][kQuads];
-  __shared__ float sum[kGroups][kQuads];
+  __shared__ float sum[kGroups][kQuads], top[kJoinThreads / 32][kHere];
   const int tid = threadIdx.x, head0 = blockIdx.y * kValues / D;
   grid_wait();
   const int4 cut = p.cut[blockIdx.x];
@@ -694,15 +695,21 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   const int g = cut.y / p.tiles, tile = cut.y % p.tiles, c1 = cut.w >> 1, parts = c1 - cut.z + 1;
   if (head0 >= p.group - tile * kHeads) return;               // heads past the group's
   auto slot = [&](int i) { return 2 * static_cast<long long>(cut.z + i) + (i == 0 ? cut.w & 1 : 0); };
-  for (int f = tid; f < parts * kHere; f += kJoinThreads)
-    ml[f / kHere][f % kHere] =
-        reinterpret_cast<const float2*>(p.part_ml)[slot(f / kHere) * kHeads + head0 + f % kHere];
+  float most = -INFINITY;                                     // of head tid % kHere
+  for (int f = tid; f < parts * kHere; f += kJoinThreads) {
+    const float2 x = reinterpret_cast<const float2*>(p.part_ml)[slot(f / kHere) * kHeads + head0 + f % kHere];
+    ml[f / kHere][f % kHere] = x;
+    most = fmaxf(most, x.x);
+  }
+#pragma unroll
+  for (int o = 16; o >= kHere; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (tid % 32 < kHere) top[tid / 32][tid % 32] = most;
   __syncthreads();
   const int quad = tid % kQuads, group = tid / kQuads;
   const int hc = quad * 4 / D;                                // this thread's head of kHere
-  float mx = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) mx = fmaxf(mx, ml[i][hc].x);
+  float mx = top[0][hc];
+#pragma unroll
+  for (int i = 1; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, top[i][hc]);
   const float base = mx == -INFINITY ? 0.f : mx;
   const float4* from = reinterpret_cast<const float4*>(p.part_o) + blockIdx.y * kQuads + quad;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -783,11 +790,12 @@ cudaError_t launch_shape(const AttnArgs& p, const Plan& q, cudaStream_t st) {
   e = cudaGetLastError();
   if (e != cudaSuccess || !q.split) return e;
   const unsigned x = static_cast<unsigned>(q.cut);
+  constexpr int kAll = 8 * NG * D;                            // values of a row
+  if (q.rows * (kAll / 32) <= 4 * kSMs)
+    return launch_after(attn_join_kernel<T, D, NG, 32>, dim3(x, kAll / 32), dim3(kJoinThreads), 0, st, p);
   if (q.rows * 8 <= q.grid)
-    return launch_after(attn_join_kernel<T, D, NG, 128>, dim3(x, 8 * NG * D / 128), dim3(kJoinThreads),
-                        0, st, p);
-  return launch_after(attn_join_kernel<T, D, NG, 512>, dim3(x, 8 * NG * D / 512), dim3(kJoinThreads), 0,
-                      st, p);
+    return launch_after(attn_join_kernel<T, D, NG, 128>, dim3(x, kAll / 128), dim3(kJoinThreads), 0, st, p);
+  return launch_after(attn_join_kernel<T, D, NG, 512>, dim3(x, kAll / 512), dim3(kJoinThreads), 0, st, p);
 }
 
 template <typename T>
