@@ -118,6 +118,18 @@ def test_cut_rows_of_other_shapes(D, HQ, HKV, lens):
     check(x, run(x, window=1500, num_sinks=9), want)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("HQ,HKV", [(17, 1), (25, 1), (32, 1), (48, 1), (66, 2), (64, 1)])
+@pytest.mark.parametrize("lens", [[200, 3, 0, 33], [2600]])
+def test_many_heads_to_a_key_value_head(D, HQ, HKV, lens):
+    x = make(lens, HQ, HKV, D, 16, seed=HQ)
+    want = expect(x, 70, 3)
+    check(x, run(x, window=70, num_sinks=3), want)
+    x = make(lens, HQ, HKV, D, 16, FP16, seed=HQ + D)
+    want = expect(x)
+    check(x, run(x), want)
+
+
 def test_without_new_rows_reads_the_cache_only():
     x = make([1, 20, 333], 8, 2, 128, 16)
     del x["k"], x["v"]
