@@ -25,9 +25,6 @@ _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
 def _gdn():
-    loaded = sys.modules.get("gdn_b200")
-    if loaded is not None:                               # a user's program imports it once
-        return loaded
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                        "flashinfer-competition-codebase_b200")
     if pkg not in sys.path:
