@@ -888,7 +888,8 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
     p.part_ml = p.part_o + static_cast<size_t>(2 * p.grid) * heads_of(p.group, D) * D;
     p.by_row = plan.rows <= plan.grid;
   }
-  p.twin = p.k_page == p.v_page && p.k_tok == p.v_tok;
+  // a token's row lies at the same offset in both caches
+  p.twin = p.k_page == p.v_page && p.k_tok == p.v_tok && (HKV == 1 || p.k_head == p.v_head);
   div_constants(static_cast<uint32_t>(page_size), p.page_mul, p.page_shift);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == GDN_DTYPE_BF16 ? launch<__nv_bfloat16>(p, D, plan, st) : launch<__half>(p, D, plan, st);
