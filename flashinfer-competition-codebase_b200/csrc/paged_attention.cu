@@ -182,6 +182,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return r;
 }
 
+// Weights are held as 2^kUp exp(x - m), l and o with them: in fp16 exp(x - m) itself would be
+// subnormal from 2^-14 of the largest on and lost below 2^-25, which 131072 tokens beside a larger one
+// add up to 0.4%; 2^15 of it is lost below 2^-40.
+template <typename T> constexpr float kUp = std::is_same_v<T, __half> ? 15.f : 0.f;
+
 // c[16 x 8] += a[16 x 16] b[16 x 8]
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -218,8 +223,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // so a group of up to 8 query heads fills the instruction, where queries as rows would
 // leave half of it empty, and the accumulators of O take D / 16 x 4 registers.  The scores'
 // accumulator layout becomes the second product's operand by an 8 x 8 transpose in
-// registers.  p is rounded to the tensors' type for that product (its own sum l is not):
-// the rounding is that of the values it multiplies, at most half a step of each weight.
+// registers.  p is rounded to the tensors' type for that product (its own sum l is not), which
+// takes operands of one type: at most half a step of each weight, as much as the values
+// carry themselves.
 //
 // Every warp streams its own tiles of 16 or 32 tokens through its own ring of kStages
 // buffers in shared memory with asynchronous copies, so the main loop has no CTA barrier.
@@ -527,10 +533,11 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
         m[n][0] = m0;
         m[n][1] = m1;
       }
+      const float s0 = b0 - kUp<T>, s1 = b1 - kUp<T>;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        const float p0 = exp2_fast(y[t][n][0] - b0), p1 = exp2_fast(y[t][n][1] - b1);
-        const float p2 = exp2_fast(y[t][n][2] - b0), p3 = exp2_fast(y[t][n][3] - b1);
+        const float p0 = exp2_fast(y[t][n][0] - s0), p1 = exp2_fast(y[t][n][1] - s1);
+        const float p2 = exp2_fast(y[t][n][2] - s0), p3 = exp2_fast(y[t][n][3] - s1);
         l[n][0] += p0 + p2;
         l[n][1] += p1 + p3;
         pb[t][n][0] = transpose8(pack2<T>(p0, p1));
@@ -609,7 +616,7 @@ attn_decode_kernel(const __grid_constant__ AttnArgs p) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) c[w] *= inv;
         if (writes && p.lse)
-          p.lse[out0 + h] = lt == 0.f ? -INFINITY : (base + log2f(lt)) * 0.6931471805599453f;
+          p.lse[out0 + h] = lt == 0.f ? -INFINITY : (base + (log2f(lt) - kUp<T>)) * 0.6931471805599453f;
       } else if (writes) {
         *reinterpret_cast<float2*>(p.part_ml + (slot * kHeads + h) * 2) = make_float2(mx, lt);
       }
@@ -743,7 +750,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   const int d = (blockIdx.y * kValues + quad * 4) % D;
   reinterpret_cast<uint2*>(p.out)[(r * D + d) / 4] =
       make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-  if (d == 0 && p.lse) p.lse[r] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+  if (d == 0 && p.lse) p.lse[r] = l == 0.f ? -INFINITY : (base + (log2f(l) - kUp<T>)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
