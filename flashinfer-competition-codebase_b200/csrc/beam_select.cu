@@ -168,8 +168,9 @@ struct ExpSum {
   }
 };
 
-// Any two different logits this large are so far apart that only the largest counts.
-constexpr float kHuge = 1e30f;
+// Two different logits from here on are 64 or more apart, so only the largest counts; below, m log2 e
+// as rounded is off by 32 at most, so that sums relative to it stay within fp32.
+constexpr float kHuge = 536870912.f;   // 2^29
 
 // One place of a list.  Few lanes of a warp ask at a time, so each asks for itself.
 __device__ __forceinline__ int next_place(int* count) {
