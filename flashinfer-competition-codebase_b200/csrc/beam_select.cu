@@ -31,6 +31,7 @@ constexpr int kList = 1024;      // vectors, then candidates, that a slice gathe
 constexpr int kMergeThreads = 512;
 constexpr int kHeadItems = 256;  // of the merge's bound, at most 256
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLn2 = 0.69314718055994530942;
 
 struct BeamArgs {
   const void* logits;
@@ -40,7 +41,8 @@ struct BeamArgs {
   int32_t* parents;
   float* out_scores;
   unsigned long long* keys;   // workspace [rows, slices, n]: keys, descending, 0 = none
-  float2* sums;               // workspace [rows, slices]: m, sum exp(x - m)
+  float2* sums;               // workspace [rows, slices]: m, sum 2^(x log2 e - reference(m)), or, of
+                              // |m| > kHuge, how many logits are m
   long long stride_batch, stride_beam;
   int B, K, V, n, eos, slices;
   uint32_t per_mul, per_shift;   // division by slices n
@@ -128,7 +130,8 @@ struct SliceShared {
   unsigned long long list[kList];  // keys of candidates
   float red[kWarps];
   float top[32];                   // its own place: red is written again without a barrier between
-  float sum[kWarps];
+  double sum[kWarps];
+  double folded[kThreads];         // each thread's sum but for its chains
   int scan[kWarps];
   unsigned long long best[kWarps];
   float sample[kThreads];        // of the keys, where they overflow
@@ -155,11 +158,12 @@ struct ExpSum {
     unpack(t, a, b);
     asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s[chain]) : "l"(pack(exp2_fast(a), exp2_fast(b))));
   }
-  __device__ __forceinline__ void scale(float f) {
+  __device__ __forceinline__ void scale(float f) {     // f a power of two: exact
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(s[i]) : "l"(pack(f, f)));
   }
+  __device__ __forceinline__ void clear() { s[0] = s[1] = 0ull; }
   __device__ __forceinline__ float total() const {
     float a, b, c, d;
     unpack(s[0], a, b);
@@ -171,6 +175,16 @@ struct ExpSum {
 // Two different logits from here on are 64 or more apart, so only the largest counts; below, m log2 e
 // as rounded is off by 32 at most, so that sums relative to it stay within fp32.
 constexpr float kHuge = 536870912.f;   // 2^29
+
+// The whole number c that a maximum m's exponentials are taken relative to, as 2^(x log2 e - c):
+// changing it, as the maximum grows or slices meet, scales a sum by a power of two, without an error.
+__device__ __forceinline__ float reference(float m) {
+  return rintf(fminf(fmaxf(m, -kHuge), kHuge) * kLog2e);
+}
+// 2^d for a whole d <= 0, 0 below the normal numbers
+__device__ __forceinline__ float power_of_two(float d) {
+  return __int_as_float((static_cast<int>(fmaxf(d, -127.f)) + 127) << 23);
+}
 
 // One place of a list.  Few lanes of a warp ask at a time, so each asks for itself.
 __device__ __forceinline__ int next_place(int* count) {
@@ -314,9 +328,17 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
     for (int w = 1; w < kWarps; ++w) bound = fminf(bound, sh.top[w]);
   }
   unsigned long long* out = p.keys + (static_cast<long long>(row) * p.slices + slice) * p.n;
-  // s = sum of 2^(x log2 e - c), c = m log2 e as rounded (within +-kHuge), in four chains
-  float c0 = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
+  // The sum of 2^(x log2 e - c0), in four chains of at most 32 additions (kFold batches), then in 64 bits in
+  // shared memory, where it takes no registers from the loop (with it there 44.8 us instead of
+  // 43.5 for 64 x 8 rows of 151936 bf16 logits; with chains as long as the slice, whose error grows with it, 43.1).
+  constexpr int kFold = 4;
+  float c0 = reference(m);
   ExpSum sums;
+  sh.folded[tid] = 0.0;
+  auto fold = [&]() {
+    sh.folded[tid] += sums.total();
+    sums.clear();
+  };
   bound = fmaxf(bound, -FLT_MAX);   // vectors of -inf alone never count
   auto set_aside = [&](const V& w, int c) {
     const int at = next_place(&sh.count);
@@ -325,10 +347,12 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
       sh.at[at] = c;
     }
   };
+  // A thread keeps its reference until a logit is 7.5 binades above it (4 binades: 44.8 us), since some
+  // lane's maximum grows in nearly every batch.
   auto raise = [&](float top) {
-    m = top;
-    const float c1 = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e, f = exp2_fast(c0 - c1);
+    const float c1 = reference(top), f = power_of_two(c0 - c1);
     sums.scale(f);
+    sh.folded[tid] *= f;
     c0 = c1;
   };
   for (int j = 0;; ++j) {
@@ -340,13 +364,15 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
       if (t >= bound) set_aside(v[k], v0 + (j + k * batches) * kThreads + tid);
       top = fmaxf(top, t);
     }
-    if (top > m) raise(top);
+    m = fmaxf(m, top);
+    if (top > (c0 + 7.5f) * static_cast<float>(kLn2)) raise(top);
     const unsigned long long minus_c = ExpSum::pack(-c0, -c0);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
 #pragma unroll
       for (int e = 0; e < E; e += 2) sums.add(e / 2 % 2, v[k].get(e), v[k].get(e + 1), minus_c);
     if (j + 1 >= batches) break;
+    if (j % kFold == kFold - 1) fold();
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) v[k] = vector(next[k]);
   }
@@ -357,15 +383,18 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   m = sh.red[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.red[w]);
-  const float held = fminf(fmaxf(m, -kHuge), kHuge), c1 = held * kLog2e;
-  float part = sums.total() * exp2_fast(c0 - c1);
+  fold();
+  double part = sh.folded[tid] * power_of_two(c0 - reference(m));
   const int e0 = v0 * E, e1 = min(p.V, v1 * E);   // the slice's tokens
-  if (held != m && isfinite(m)) {
-    part = 0.f;
+  if (fabsf(m) > kHuge && isfinite(m)) {
+    int equal = 0;
+    bool broken = false;
     for (int t = e0 + tid; t < e1; t += kThreads) {
       const float y = to_f(x[t]);
-      part += isnan(y) ? NAN : y == m ? 1.f : 0.f;
+      equal += y == m;
+      broken |= isnan(y);
     }
+    part = broken ? NAN : equal;
   }
   part = warp_sum(part);
   if (lane == 0) sh.sum[warp] = part;
@@ -373,8 +402,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_slice_kernel(const BeamArgs 
   if (tid == 0) {
     double s = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += static_cast<double>(sh.sum[w]);
-    if (held == m) s *= static_cast<double>(exp2f(-fmaf(held, kLog2e, -c1)));   // what c's rounding took
+    for (int w = 0; w < kWarps; ++w) s += sh.sum[w];
     p.sums[static_cast<long long>(row) * p.slices + slice] = make_float2(m, static_cast<float>(s));
   }
   // a sharper bound from up to 256 of the vectors set aside, as before: whole warps of them,
@@ -531,12 +559,12 @@ __device__ __forceinline__ MergeItem make_item(double score, int beam, unsigned 
                                        (key >> 32) << kTokenBits | (key & tokens)};
 }
 
-// ln(t) for t >= 1: the fraction's logarithm in fp32 (6e-8), the exponent's in 64 bits
+// ln(t) for normal t: the fraction's logarithm in fp32 (6e-8), the exponent's in 64 bits
 __device__ __forceinline__ double ln_sum(double t) {
   const unsigned long long u = __double_as_longlong(t);
   const int e = static_cast<int>(u >> 52) - 1023;
   const double f = __longlong_as_double((u & 0x000fffffffffffffull) | 0x3ff0000000000000ull);
-  return e * 0.69314718055994530942 + static_cast<double>(logf(static_cast<float>(f)));
+  return e * kLn2 + static_cast<double>(logf(static_cast<float>(f)));
 }
 
 // over a group of N lanes; other groups of the warp may have left the loop
@@ -615,16 +643,22 @@ __global__ void __launch_bounds__(kMergeThreads, 2) beam_merge_kernel(const __gr
     if (on)
       for (int s = s8 + 8; s < p.slices; s += 8) m = fmaxf(m, sums[s].x);
     m = group_max<8>(m);
+    const bool huge = fabsf(m) > kHuge;
+    const float c = reference(m);
     auto term = [&](float2 ms) {
-      return ms.x > -INFINITY || isnan(ms.y)
-                 ? static_cast<double>(ms.y) * static_cast<double>(exp2_fast((ms.x - m) * kLog2e))
-                 : 0.0;
+      if (!(ms.x > -INFINITY || isnan(ms.y))) return 0.0;
+      const float f = huge || fabsf(ms.x) > kHuge ? (ms.x == m || isnan(ms.y) ? 1.f : 0.f)
+                                                  : power_of_two(reference(ms.x) - c);
+      return static_cast<double>(ms.y) * f;
     };
     double t = term(first);
     if (on)
       for (int s = s8 + 8; s < p.slices; s += 8) t += term(sums[s]);
     t = group_sum<8>(t);
-    if (on && isfinite(m) && t >= 0.5 && t < 1e300) l = m + ln_sum(t);
+    // sum 2^(x L - c) with L = log2 e as rounded is e^(m (L ln 2 - 1)) 2^-c sum e^x, near enough for x
+    // that are not far below m
+    if (on && isfinite(m) && t > 0.0 && t < 1e300)
+      l = (huge ? static_cast<double>(m) : c * kLn2 - m * (kLog2e * kLn2 - 1.0)) + ln_sum(t);
     if (s8 == 0) lse[i8] = l;
   }
   __syncthreads();

@@ -21,7 +21,7 @@ inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   return pa < pb + nb && pb < pa + na;
 }
 
-__device__ __forceinline__ float warp_sum(float x) {
+template <typename T> __device__ __forceinline__ T warp_sum(T x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;

@@ -1,9 +1,17 @@
-"""beam_select on rows of large finite logits.
+"""beam_select's log-sum-exp: rows of large finite logits, long rows, rows that rise.
 
-Tolerance: that of test_beam_select_gpu, whose c is m log2 e as rounded.  From |m| = 2^23 on that is off
-by up to |m| 2^-23, 32 at most, of which a term's exponent carries 2^-24 more.  From 2^29 on different
-logits are 64 or more apart: only the largest counts.
+Tolerance, in units of 2^-24 of the score's absolute error.  A term's exponent x log2 e - c is less than 8
+and, below, at most |x - m| log2 e + 1/2 in size.  It is rounded once, by half a step, so by at most
+max(4, |x - m| log2 e + 1/2) units, times ln 2; log2 e itself is off by 0.22 relative; and the
+weighted mean of |x - m| is at most ln V: 1.22 ln V + 3.2 < 25.3 for V <= 2^26.  The exponential 4; a
+chain of at most 32 additions and the two that join four chains 34; everything behind is in 64 bits, scaled by
+powers of two, but a slice's sum, stored in 32 (1), and the logarithm of the fraction (2).  Together
+less than 67 units, 4e-6.
+From |m| = 2^23 on c is no longer within 1/2 of m log2 e but within |m| 2^-23, up to 32: 2^-24 of
+that more, times ln 2.  From 2^29 on different logits are 64 or more apart: only the largest counts.
 """
+
+import math
 
 import pytest
 import torch
@@ -44,3 +52,52 @@ def test_large_finite_logits(dtype, top, sign):
     check_scores(x, s, 6, got)
     for r in range(6):
         assert (int(got[1][0, r]), int(got[0][0, r])) == cands[r][1:], (r, cands[:6])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("drop", [0.125, 1.0, 2.3, 7.0])
+@pytest.mark.parametrize("V", [151936, 2**20 + 3])
+def test_long_slices_of_equal_terms(dtype, drop, V):
+    """So many rows that each is one slice: equal terms round the same way at every addition."""
+    row = torch.full((V,), -drop)
+    row[:2048:4] = 0.0                                  # the first vector of every thread holds one
+    x = row.to(dtype).cuda().expand(224, 8, V)
+    s = -torch.arange(8.0).expand(224, 8).contiguous().cuda()
+    toks, pars, news = gdn_b200.beam_select(x, s, num_selected=8)
+    want = s[0].double().cpu() - torch.logsumexp(row.to(dtype).double(), 0)
+    assert bool((pars == 0).all()) and bool((toks == torch.arange(0, 32, 4, device="cuda")).all())
+    err = (news.cpu().double() - want[0]).abs().max()
+    assert float(err) <= TOL + abs(float(want[0])) * 2.0**-24, float(err)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B", [1, 224])
+def test_rising_rows(dtype, B):
+    """The running maximum grows all along the row: the sums are scaled at every step."""
+    V = 300007
+    row = torch.linspace(-30.0, 0.0, V).to(dtype)
+    x = row.cuda().expand(B, 8, V)
+    s = torch.zeros(B, 8).cuda()
+    toks, pars, news = gdn_b200.beam_select(x, s, num_selected=3)
+    first = int((row == row.max()).nonzero()[0])
+    want = float(row.double().max() - torch.logsumexp(row.double(), 0))
+    assert int(toks[0, 0]) == first and int(pars[0, 0]) == 0
+    assert float((news[:, 0].cpu().double() - want).abs().max()) <= TOL + abs(want) * 2.0**-24
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_slices_on_both_sides_of_the_largest_exact_size(sign):
+    """2^29 in one slice, the next larger or smaller logits in the others."""
+    x = torch.full((1, 1, 40000), sign * 2.0**29)
+    x[..., 20000:] += -64.0 if sign > 0 else -128.0
+    x, s = x.cuda(), torch.zeros(1, 1).cuda()
+    check_scores(x, s, 2, gdn_b200.beam_select(x, s, num_selected=2))
+
+
+def test_equal_rows_tie_in_long_slices():
+    x = (torch.randn(1, 1, 151937, generator=torch.Generator().manual_seed(3)) * 2.5)
+    x = x.to(torch.bfloat16).cuda().expand(300, 8, 151937).clone()     # rows begin anywhere
+    toks, pars, news = gdn_b200.beam_select(x, torch.zeros(300, 8, device="cuda"))
+    assert bool((news == news[0]).all()) and bool((toks == toks[0]).all())
+    assert pars[0].tolist() == list(range(8)) and len(set(toks[0].tolist())) == 1
+    assert math.isfinite(float(news[0, 0]))
