@@ -64,12 +64,13 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& p, int n) {   // n: its 
 //
 // A "row" is (sequence, key-value head, tile of 8, 16 or 24 of its query heads); it has
 // ceil(vis / block) blocks of tokens, at least one.  All rows' blocks in a line (sequence,
-// row, block) are cut into equal shares, one per CTA, so ragged batches, one long sequence
-// and many short ones all load the GPU evenly.  A CTA that has all of a row writes its
-// output; a row that is cut leaves partial sums (at most two per CTA: its first and its last
-// row), which attn_join_kernel adds up in a fixed order.  The cut depends on lens alone, so
-// no counters or flags have to be kept in memory.  In a call whose rows all are short
-// none is cut (cut == null): a row is then one unit of the line.
+// row, block) are cut into equal shares, one per CTA, so ragged batches and one long sequence
+// load the GPU evenly.  A CTA that has all of a row writes its output; a row that is cut leaves
+// partial sums (at most two per CTA: its first and its last row), which attn_join_kernel adds
+// up in a fixed order.  The cut depends on lens alone, so no counters or flags have to be kept
+// in memory.  In a call whose rows cannot be long, going by its table's width and its window,
+// none is cut (cut == null): a row is then one unit of the line, and plan_of says how far from
+// an even share that may be.
 
 constexpr int kWarps = 4;        // that take tiles of their own, alone or as teams
 
@@ -767,11 +768,15 @@ int heads_of(int group, int D) {
 int block_of(int D) { return D == 64 ? Shape<64>::kBlock : D == 128 ? Shape<128>::kBlock : Shape<256>::kBlock; }
 int resident(int D) { return D == 64 ? Shape<64>::kResident : D == 128 ? Shape<128>::kResident : Shape<256>::kResident; }
 
-// Rows are not cut where that leaves no CTA more than about 4 blocks over an even share: less
-// than the cut's partial sums and the join cost.  Not cut / cut: 1 row of 100 tokens of 128 dims
-// 5.3 / 7.0 us, of 512 tokens 10.2 / 7.1 us; 512 rows of 256 tokens 14.4 / 18.0 us, of 500
-// tokens 27.8 / 30.0 us; 300 rows of 330 tokens of 64 dims 12.3 / 14.8 us; of 256 dims 75 rows 11.5
-// / 15.0 us, 150 rows 20.2 / 19.0 us.
+// Rows are left whole, without partial sums and a join, where neither way of sharing unevenly costs more:
+//  - rows of one length leave some CTAs without a row in the last wave; cutting them would take at most
+//    4 blocks from every CTA.  Not cut / cut: 1 row of 100 tokens of 128 dims 5.3 / 7.0 us, of 512 tokens
+//    10.2 / 7.1 us; 512 rows of 256 tokens 14.4 / 18.0 us, of 500 tokens 27.8 / 30.0 us; 300 rows of 330
+//    tokens of 64 dims 12.3 / 14.8 us; of 256 dims 75 rows 11.5 / 15.0 us, 150 rows 20.2 / 19.0 us.
+//  - the longest row the call allows beside short ones gives its CTA up to 24 blocks more than one a row.
+//    Not cut / cut, 296 rows of 128 dims, rows rising from 1 token to so many, and one such row among
+//    rows of 16 tokens: 576 tokens 22.5 / 34.8 and 18.4 / 20.5 us, 1024 30.7 / 51.2 and 24.6 / 20.5, 2048
+//    49.2 / 71.7 and 36.9 / 22.5, 8192 154 / 143 and 125 / 24.6.
 
 struct Plan {
   long long rows, grid;      // rows of a call; CTAs: what the GPU holds at once, or fewer
@@ -786,7 +791,7 @@ Plan plan_of(int B, int HQ, int HKV, int D, long long max_tokens) {
   const long long nb = max_tokens > 0 ? (max_tokens + block_of(D) - 1) / block_of(D) : 1;
   const long long most = static_cast<long long>(kSMs) * resident(D);
   const long long waves = (q.rows + most - 1) / most;
-  q.split = nb * (waves * most - q.rows) > 4 * most;
+  q.split = nb * (waves * most - q.rows) > 4 * most || waves * (nb - 1) > 24;
   const long long units = q.rows * (q.split ? nb : 1);
   q.grid = units < most ? units : most;
   q.cut = static_cast<size_t>(q.rows <= q.grid ? q.rows : q.grid);
