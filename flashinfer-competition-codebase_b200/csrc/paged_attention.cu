@@ -865,14 +865,19 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] < 0 || v_strides[i] < 0 || k_strides[i] % 8 || v_strides[i] % 8)
       return GDN_ERR_ALIGN;
-  const size_t out_bytes = static_cast<size_t>(B) * HQ * D * 2;
+  // CTAs write their rows' results while others, ahead of them or behind, still read theirs
+  const size_t out_bytes = static_cast<size_t>(B) * HQ * D * 2, new_bytes = static_cast<size_t>(B) * HKV * D * 2;
+  const size_t table_bytes = table_width > 0 ? 4 * static_cast<size_t>((B - 1) * table_stride + table_width) : 0;
   auto cache_bytes = [&](const int64_t* st) {
     return 2 * static_cast<size_t>((num_pages - 1) * st[0] + (page_size - 1) * st[1] + (HKV - 1) * st[2] + D);
   };
-  if (overlaps(output, out_bytes, q, out_bytes) ||
-      overlaps(output, out_bytes, k_cache, cache_bytes(k_strides)) ||
-      overlaps(output, out_bytes, v_cache, cache_bytes(v_strides)) || (k_new && k_cache == v_cache))
-    return GDN_ERR_ALIAS;
+  auto meets_inputs = [&](const void* x, size_t bytes) {
+    return overlaps(x, bytes, q, out_bytes) || overlaps(x, bytes, k_cache, cache_bytes(k_strides)) ||
+           overlaps(x, bytes, v_cache, cache_bytes(v_strides)) ||
+           (k_new && (overlaps(x, bytes, k_new, new_bytes) || overlaps(x, bytes, v_new, new_bytes))) ||
+           overlaps(x, bytes, block_tables, table_bytes) || overlaps(x, bytes, seq_lens, 4 * static_cast<size_t>(B));
+  };
+  if (meets_inputs(output, out_bytes) || (k_new && k_cache == v_cache)) return GDN_ERR_ALIAS;
   // no row sees more than its table holds, or its window and sinks
   const int held = table_width * page_size;
   const int max_tokens = window > 0 && window + num_sinks < held ? window + num_sinks : held;
@@ -880,6 +885,8 @@ int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cache,
   if (plan.bytes > 0 && !workspace) return GDN_ERR_NULL;
   if (!aligned(workspace, 16)) return GDN_ERR_ALIGN;
   if (workspace_bytes < plan.bytes) return GDN_ERR_SHAPE;
+  const size_t lse_bytes = static_cast<size_t>(B) * HQ * 4;
+  if (lse && (meets_inputs(lse, lse_bytes) || overlaps(lse, lse_bytes, output, out_bytes))) return GDN_ERR_ALIAS;
   AttnArgs p{};
   p.q = q; p.k = static_cast<char*>(k_cache); p.v = static_cast<char*>(v_cache);
   p.tables = block_tables; p.lens = seq_lens; p.k_new = k_new; p.v_new = v_new;

@@ -138,7 +138,8 @@ def paged_attention_decode(
     hides its tokens; one >= num_pages does too and is counted in ``bad_index_count`` (an int32
     CUDA tensor of one element), like a length beyond the table, which is cut to it.  The new
     token is seen even when its page is bad, but not stored.  The page of a sequence's last
-    token must not be shared.  C entry: ``gdn_paged_attention_decode``.
+    token must not be shared, and ``output`` not overlap an input.  C entry:
+    ``gdn_paged_attention_decode``.
     """
     made = (_calls or _torch_calls()).attend(q, k_cache, v_cache, block_tables, seq_lens, k, v, scale,
                                             window, num_sinks, output, bad_index_count)

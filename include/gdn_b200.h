@@ -498,7 +498,8 @@ GDN_API int gdn_interleave_heads(const gdn_bf16* gathered, gdn_bf16* output,
  * there are harmless).  The page of the last token must belong to this sequence alone;
  * all other pages may be shared.  `workspace`: gdn_paged_attention_workspace_bytes bytes
  * for max_tokens = table_width * page_size, or window + num_sinks where that is less;
- * 16-byte aligned, contents ignored and overwritten.  output may not overlap q or the caches.
+ * 16-byte aligned, contents ignored and overwritten.  output and lse may not overlap each other
+ * or an input.
  */
 GDN_API size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D,
                                                    int max_tokens);
