@@ -981,8 +981,8 @@ const char* gdn_strerror(int code) {
     case GDN_ERR_SHAPE: return "unsupported or inconsistent sizes (GDN: K and V must be 128, HV a multiple of H; attention: D 64, 128 or 256, HQ a multiple of HKV)";
     case GDN_ERR_ALIGN: return "misaligned pointer or stride (state and attention tensors need 16 B, GDN q/k 8 B, fp32 and int32 vectors 4 B, bf16 2 B)";
     case GDN_ERR_LAUNCH: return "CUDA kernel launch failed";
-    case GDN_ERR_ALIAS: return "buffers overlap that must be disjoint or the same";
-    case GDN_ERR_ARG: return "invalid argument value";
+    case GDN_ERR_ALIAS: return "state and new_state overlap without being the same buffer, or an output overlaps an input, or pools or pages share bytes";
+    case GDN_ERR_ARG: return "invalid argument value (GDN: rank or world out of range, eps, output indices without indices; attention: dtype, scale, window, num_sinks; beam_select: dtype, strides, eos_token)";
     case GDN_ERR_LIMIT: return "beyond a fixed maximum (gdn_decode_tp_static: channel must be 0..63; beam_select: 64 beams, 64 selected; pages: 32 pools, 4096 copy pairs)";
     default: return "unknown gdn error code";
   }
