@@ -164,7 +164,9 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def torch_calls():
     """The serving operators' calls as a CPython extension (``csrc/torch_entry.cpp``), or None
-    where it is not built for this torch and Python: the same calls then go through ctypes."""
+    where it is not built for this torch and Python or, with a warning, does not load: the same
+    calls then go through ctypes."""
+    import warnings
     from importlib.machinery import ExtensionFileLoader
     from importlib.util import module_from_spec, spec_from_file_location
 
@@ -175,8 +177,14 @@ def torch_calls():
         return None
     load()
     loader = ExtensionFileLoader("gdn_b200_torch", path)
-    module = module_from_spec(spec_from_file_location("gdn_b200_torch", path, loader=loader))
-    loader.exec_module(module)
+    try:
+        module = module_from_spec(spec_from_file_location("gdn_b200_torch", path, loader=loader))
+        loader.exec_module(module)
+    except ImportError as e:
+        warnings.warn(f"{path} does not load ({e}); the serving operators' calls go through ctypes, at "
+                      "10 us more each, until `python -m gdn_b200.build --force` has built it again",
+                      RuntimeWarning, stacklevel=2)
+        return None
     return module
 
 
