@@ -27,12 +27,6 @@ template <typename T> __device__ __forceinline__ T warp_sum(T x) {
   return x;
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
-}
-
 constexpr int kSMs = 148;
 
 // x / d for 32-bit x by multiplication with mul and shift from div_constants
