@@ -132,13 +132,18 @@ def paged_attention_decode(
     counts each sequence's tokens, the new one included.  With k, v [B,1,HKV,D] the new token's
     rows are attended to and stored into the cache at position ``seq_lens - 1``; without them
     they have to be there already.  ``window`` > 0 leaves the first ``num_sinks`` and the last
-    ``window`` tokens visible.  Returns ``(output [B,1,HQ,D], lse [B,HQ] fp32)``.
+    ``window`` tokens visible.  ``scale`` None or 0 is 1/sqrt(D), as in the GDN entries.  Returns
+    ``(output [B,1,HQ,D], lse [B,HQ] fp32)``.
 
     A row of length <= 0 is padding: zeros, lse -inf, nothing stored.  A table entry < 0
     hides its tokens; one >= num_pages does too and is counted in ``bad_index_count`` (an int32
     CUDA tensor of one element), like a length beyond the table, which is cut to it.  The new
     token is seen even when its page is bad, but not stored.  The page of a sequence's last
-    token must not be shared, and ``output`` not overlap an input.  C entry:
+    token must not be shared, and ``output`` not overlap an input.
+
+    Scores, maxima, sums and the output's sums are fp32; each softmax weight is rounded to the tensors'
+    type where it is multiplied with its value (in fp16 times 2^15, so that small ones are not lost),
+    and the output once more.  At most 65535 sequences, and B * HQ up to 2**31 // 256.  C entry:
     ``gdn_paged_attention_decode``.
     """
     made = (_calls or _torch_calls()).attend(q, k_cache, v_cache, block_tables, seq_lens, k, v, scale,
@@ -216,8 +221,8 @@ def beam_select(
     ``scores[i]``.  Returns ``(tokens, parents, new_scores)``, int32, int32 and fp32
     [B,num_selected], best first; equal scores: the lower beam, within a beam the lower token.
     Candidates without a finite score (tokens masked with -inf, beams at -inf, rows that hold
-    a NaN or +inf) are never chosen; places left over get -1, -1, -inf.  At most 64 beams and
-    64 selected.  C entry: ``gdn_beam_select``.
+    a NaN or +inf) are never chosen; places left over get -1, -1, -inf.  At most 64 beams,
+    64 selected, 2**26 tokens and 2**25 - 1 beams in all.  C entry: ``gdn_beam_select``.
     """
     made = (_calls or _torch_calls()).select(logits, scores, num_selected, finished, eos_token)
     if _made(made, "gdn_beam_select"):

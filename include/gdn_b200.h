@@ -499,7 +499,9 @@ GDN_API int gdn_interleave_heads(const gdn_bf16* gathered, gdn_bf16* output,
  * all other pages may be shared.  `workspace`: gdn_paged_attention_workspace_bytes bytes
  * for max_tokens = table_width * page_size, or window + num_sinks where that is less;
  * 16-byte aligned, contents ignored and overwritten.  output and lse may not overlap each other
- * or an input.
+ * or an input.  Scores, the softmax's maximum and sum and the output's sums are fp32; each weight
+ * is rounded to the tensors' type where it is multiplied with its value (in fp16 times 2^15), and
+ * the output once more.  B <= 65535, B * HQ <= 2^31 / 256 (GDN_ERR_SHAPE).
  */
 GDN_API size_t gdn_paged_attention_workspace_bytes(int B, int HQ, int HKV, int D,
                                                    int max_tokens);
@@ -524,7 +526,8 @@ GDN_API int gdn_paged_attention_decode(const void* q, void* k_cache, void* v_cac
  * beam are ordered by logit, equal ones by token; beams are merged by score in 64 bits,
  * equal ones by beam.  Candidates without a finite score (masked tokens at -inf, beams with
  * scores[i] = -inf, rows that hold a NaN or +inf) are never chosen; places left over get
- * token -1, parent -1, score -inf.  K <= 64, n <= 64 (GDN_ERR_LIMIT).
+ * token -1, parent -1, score -inf.  K <= 64, n <= 64 (GDN_ERR_LIMIT); V <= 2^26, B * K < 2^25
+ * (GDN_ERR_SHAPE).
  */
 GDN_API size_t gdn_beam_select_workspace_bytes(int B, int K, int V, int n);
 GDN_API int gdn_beam_select(const void* logits, int dtype, int64_t stride_batch,

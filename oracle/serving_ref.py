@@ -19,7 +19,8 @@ def attention(q, k_cache, v_cache, tables, lens, k=None, v=None, scale=None, win
     B, _, HQ, D = q.shape
     P, ps, HKV, _ = kc.shape
     width = tables.shape[1]
-    scale = 1.0 / math.sqrt(D) if not scale else scale
+    if scale is None or scale == 0:                     # 0 stands for it too, as in the GDN entries
+        scale = 1.0 / math.sqrt(D)
     out = torch.zeros(B, HQ, D, dtype=torch.float64)
     absv = torch.zeros(B, HQ, D, dtype=torch.float64)
     lse = torch.full((B, HQ), -math.inf, dtype=torch.float64)
