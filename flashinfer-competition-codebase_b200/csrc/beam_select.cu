@@ -101,8 +101,8 @@ template <typename T> struct Vec {
 // ------------------------------------------------------------------ one slice of a row
 //
 // A row's slices are counted in vectors of 16 bytes from its first token, and a row that need
-// not begin on a 16-byte boundary is read in words of 32 bits (64 x 8 rows of 151936 bf16
-// logits: 47 us instead of 42): equal rows get equal sums, bit for bit, wherever they lie, so
+// not begin on a 16-byte boundary is read in words of 32 bits (64 x 8 rows of 151937 bf16
+// logits: 48 us, of 151936 43.5): equal rows get equal sums, bit for bit, wherever they lie, so
 // that equal beams tie.
 //
 // One pass over the slice.  Every thread keeps its own running maximum and its sum of
@@ -114,13 +114,14 @@ template <typename T> struct Vec {
 // reaches that is ranked.  Raising T on the way takes barriers, which cost more than it saves
 // (64 x 8 rows of 151936 logits: 47 us with, 43 without).
 //
-// Bound: the issue of instructions.  The exponentials alone come near HBM for 16-bit logits
-// (12.3 logits a clock and SM at the measured copy rate, of 16 exponentials), so an element
-// costs one unpack, one exponential, half of a packed multiply-add and of a packed addition,
-// and parts of packed maxima: 94 instructions for a vector of eight with all that is set
-// aside.  64 x 8 rows of 151936 bf16 logits, a tenth finished: 39 us (140 MB, 3.6 TB/s; a copy's
-// rate would read them in 21).  8 x 32 rows of 50257 fp32, a
-// quarter finished: 15 us (39 MB, 2.6 TB/s; 14 with rows padded to begin on 16 bytes).
+// Bound: of 16-bit logits no one unit, but two near each other: 90 warp instructions are issued for a vector of
+// eight (counted, with sampling, what is set aside and ranking in them; the sums take 24), and one exponential a
+// logit, of which an SM does 16 a clock.  64 x 8 rows of 151936 bf16 logits, a tenth finished: 39 us (140 MB,
+// 3.6 TB/s; a copy's rate would read them in 21), in which the SMs work 81% of the time (906 slices on 592
+// places) and then issue in 62% and have the exponential pipe busy in 60% of the cycles, 26 of 64 warps
+// resident.  8 x 32 rows of 50257 fp32, a quarter finished: 16 us (39 MB, 2.4 TB/s) in one wave of 576 slices: the life
+// of one, sample, five batches, gathering and ranking, 113 instructions for a vector of four; issue
+// 56%, exponentials 38% of the cycles.
 // Tried there without gain: three to eight CTAs an SM (41 to 72 us), batches of 2 and 8, a ring
 // of asynchronous copies through shared memory (50), places by ballots (55).
 

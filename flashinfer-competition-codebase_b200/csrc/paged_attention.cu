@@ -235,8 +235,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 //
 // Bound: HBM; a cached byte takes part in one operation for each head of its group, far below
 // the tensor cores' rate, so the warp-level instructions, whose operands need no staging
-// through tensor memory, are enough.  64 sequences of 820 to 8191 tokens, 32 heads over 8 of 128: 242 us
-// (1.59 GB, 6.56 TB/s, all of a copy's rate).  One of 131072 tokens, 16 heads over 2 of 256: 51 us
+// through tensor memory, are enough.  64 sequences of 820 to 8191 tokens, 32 heads over 8 of 128: 245 us
+// (1.59 GB, 6.48 TB/s, 0.98 of a copy's rate).  One of 131072 tokens, 16 heads over 2 of 256: 51 us
 // (268 MB, 5.2 TB/s): 46 and the join, whose latency nothing hides.  One of 100 tokens: 5.3 us,
 // the latency of a launch and five dependent reads.
 //
