@@ -7,8 +7,9 @@ weighted mean of |x - m| is at most ln V: 1.22 ln V + 3.2 < 25.3 for V <= 2^26. 
 chain of at most 32 additions and the two that join four chains 34; everything behind is in 64 bits, scaled by
 powers of two, but a slice's sum, stored in 32 (1), and the logarithm of the fraction (2).  Together
 less than 67 units, 4e-6.
-From |m| = 2^23 on c is no longer within 1/2 of m log2 e but within |m| 2^-23, up to 32: 2^-24 of
-that more, times ln 2.  From 2^29 on different logits are 64 or more apart: only the largest counts.
+From |m| = 2^23 on c, and the limit above which a thread takes another, are rounded by up to half a step
+of |m| log2 e each: the exponent is up to |m| 2^-23 log2 e larger, of which the rounding takes 2^-24, times
+ln 2.  From 2^29 on different logits are 64 or more apart: only the largest counts.
 """
 
 import math
